@@ -435,6 +435,101 @@ int hca_fp8_grouped_gemm(void* out, int64_t out_stride_tok, int64_t out_stride_g
                          const float* w_scale, int32_t num_tokens, int32_t num_groups, int32_t n,
                          int32_t k, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* The rest of a decode step: products on a few rows, logits                */
+/* ---------------------------------------------------------------------- */
+/* Operators of the library's own; the reference leaves them to vLLM.  */
+
+/* Products with 4-bit weights and group scales, for a few rows of x:
+ *   out[t, n] = sum_k x[t, k] * (q[n, k] - z[n, k / g]) * s[n, k / g]
+ * x [T, K] and out [T, N] bf16, or fp16 with is_fp16; rows of x 16-byte
+ * aligned (x_stride a multiple of 8).  q [N, K / 2] contiguous, 16-byte
+ * aligned, the low nibble of a byte the even k; scales [N, K / g] of x's
+ * type; zeros [N, K / g] whole numbers 0..255, NULL = 8 everywhere.
+ * g = group_size 32, 64 or 128, dividing K.  Products and sums in fp32, one
+ * rounding.  Any T is right; the weights are read again for every 32 rows. */
+int hca_w4_linear(void* out, int64_t out_stride, const void* x, int64_t x_stride, const uint8_t* q,
+                  const void* scales, const uint8_t* zeros, int32_t num_tokens, int32_t n, int32_t k,
+                  int32_t group_size, int32_t is_fp16, void* stream);
+
+/* Router of a mixture-of-experts layer.  logits = x Wr^T in fp32 (x bf16
+ * [T, H], rows 16-byte aligned; router [E, H] contiguous bf16, or fp32 with
+ * router_fp32); score = softmax(logits), or sigmoid(logits) with sigmoid.
+ * ids[t] = the top_k experts with the largest score + router_bias (fp32 [E]
+ * or NULL), largest first, ties to the lower expert, NaN last;
+ * weights[t, j] = the score (without the bias), divided by the chosen ones'
+ * sum with renormalize (0 where that sum is 0), times routed_scale.  Rows whose
+ * token_mask byte is 0 get ids -1 and weights 0.  E <= 512, top_k <= 16 and
+ * <= E, H a multiple of 32. */
+int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride, const void* router,
+                  int32_t router_fp32, const float* router_bias, const uint8_t* token_mask,
+                  int32_t num_tokens, int32_t num_experts, int32_t hidden, int32_t top_k,
+                  int32_t sigmoid, int32_t renormalize, float routed_scale, void* stream);
+
+/* Weight formats of the expert matrices. */
+#define HCA_WEIGHT_BF16 0 /* [E, N, K] bf16 */
+#define HCA_WEIGHT_FP8 1  /* e4m3 with fp32 scales [E, ceil(N / 128), ceil(K / 128)] of 128 x 128 blocks */
+#define HCA_WEIGHT_W4 2   /* 4-bit codes [E, N, K / 2], bf16 scales [E, N, K / g], zeros or NULL, as hca_w4_linear */
+
+/* Experts of a mixture-of-experts layer for a few tokens:
+ *   out[t] = sum_j weights[t, j] * W2_e (silu(W1_e x_t) * (W3_e x_t)), e = ids[t, j]
+ * plus the shared expert's W2 (silu(W1 x) * (W3 x)) where shared_inner > 0.
+ * w13 [E, 2 I, H] (W1 over W3), w2 [E, H, I], shared13 [2 Is, H], shared2
+ * [H, Is], all of one format, contiguous, 16-byte aligned.  ids outside
+ * [0, E) are skipped; an id may repeat.  A row whose token_mask byte is 0
+ * takes no part and its out is 0.  I, Is and H multiples of 32 (and of the
+ * group).  The gated product is rounded to bf16 once, with its weight in it;
+ * everything else is summed in fp32.  Any T; passes of 64 tokens.
+ * workspace: hca_moe_workspace_bytes(...) bytes, 16-byte aligned, not to be
+ * shared by calls that are not ordered on one stream. */
+int64_t hca_moe_workspace_bytes(int32_t num_tokens, int32_t top_k, int32_t inner, int32_t shared_inner);
+int hca_moe_experts(void* out, int64_t out_stride, const void* x, int64_t x_stride, const int32_t* ids,
+                    const float* weights, const uint8_t* token_mask, int32_t format, int32_t group_size,
+                    const void* w13, const void* w13_scale, const uint8_t* w13_zero, const void* w2,
+                    const void* w2_scale, const uint8_t* w2_zero, const void* shared13,
+                    const void* shared13_scale, const uint8_t* shared13_zero, const void* shared2,
+                    const void* shared2_scale, const uint8_t* shared2_zero, int32_t num_tokens,
+                    int32_t num_experts, int32_t hidden, int32_t inner, int32_t shared_inner,
+                    int32_t top_k, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* hca_moe_route and hca_moe_experts in one call, the routing in the workspace. */
+int hca_moe_decode(void* out, int64_t out_stride, const void* x, int64_t x_stride, const void* router,
+                   int32_t router_fp32, const float* router_bias, int32_t sigmoid, int32_t renormalize,
+                   float routed_scale, const uint8_t* token_mask, int32_t format, int32_t group_size,
+                   const void* w13, const void* w13_scale, const uint8_t* w13_zero, const void* w2,
+                   const void* w2_scale, const uint8_t* w2_zero, const void* shared13,
+                   const void* shared13_scale, const uint8_t* shared13_zero, const void* shared2,
+                   const void* shared2_scale, const uint8_t* shared2_zero, int32_t num_tokens,
+                   int32_t num_experts, int32_t hidden, int32_t inner, int32_t shared_inner,
+                   int32_t top_k, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Types of logits. */
+#define HCA_LOGITS_FP32 0
+#define HCA_LOGITS_BF16 1
+#define HCA_LOGITS_FP16 2
+
+/* Biases, penalties for repeated tokens and a grammar mask on logits [rows,
+ * vocab], in place, in fp32 with one rounding:
+ *   x += bias of v;  v in prompt or answer: x > 0 ? x / repetition : x * repetition
+ *   v n > 0 times in the answer: x -= frequency * n + presence
+ *   bit v of the row's mask 0: x = -inf, whatever it was
+ * Row i belongs to request req_index[i] (NULL: request i; outside
+ * [0, num_reqs): the row is left as it is).  token_ids [num_reqs, >= width]
+ * holds a request's prompt and then its answer: tokens [0, prompt_lens[i]) and
+ * [prompt_lens[i], seq_lens[i]) for row i (lengths are by row, so the rows of
+ * a request's drafts can see different lengths; cut to token_width).
+ * repetition, frequency, presence fp32 by request, NULL = none; bias_ids /
+ * bias_values [num_reqs, bias_width]; of an id listed twice the later entry
+ * counts.  Ids outside [0, vocab) are skipped in both tables.
+ * allowed_bitmask int32 [rows, ceil(vocab / 32)], bit v % 32 of word v / 32. */
+int hca_logit_penalties(void* logits, int64_t logits_stride, int32_t type, const int32_t* req_index,
+                        int32_t num_reqs, const int32_t* token_ids, int64_t token_stride,
+                        int32_t token_width, const int32_t* prompt_lens, const int32_t* seq_lens,
+                        const float* repetition, const float* frequency, const float* presence,
+                        const int32_t* bias_ids, const float* bias_values, int64_t bias_stride,
+                        int32_t bias_width, const int32_t* allowed_bitmask, int64_t allowed_stride,
+                        int32_t num_rows, int32_t vocab, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

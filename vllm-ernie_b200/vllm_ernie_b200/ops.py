@@ -8,6 +8,8 @@ only its documented outputs.  A failing status raises ``HcaError``.
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from ._lib import call, lib
@@ -532,3 +534,315 @@ def quantize_weight_block_fp8(w: torch.Tensor, block: int = 128):
     scale = torch.exp2(e)
     q = (blocks / scale[..., :, None, :, None]).clamp(-448.0, 448.0).to(FP8)
     return q.view(*lead, nb * block, k)[..., :n, :].contiguous(), scale.contiguous()
+
+
+# ---------------------------------------------------------------------------
+# the rest of a decode step: products on a few rows, logits
+# ---------------------------------------------------------------------------
+
+W4_GROUPS = (32, 64, 128)
+
+
+def _need(cond: bool, what: str) -> None:
+    if not cond:
+        raise ValueError(what)
+
+
+def _check_here(*ts: torch.Tensor | None) -> None:
+    """Every tensor on the current device, whose current stream is used."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.get_device() != here):
+            raise ValueError("libhca_b200 ops take CUDA tensors of the current device")
+
+
+def _rows_out(x: torch.Tensor, n: int, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
+    _check_here(out)
+    _need(out.shape == (x.shape[0], n) and out.dtype == x.dtype and (n == 1 or out.stride(1) == 1),
+          f"out must be {x.dtype} [{x.shape[0]}, {n}] with contiguous rows")
+    return out
+
+
+def _check_rows(x: torch.Tensor) -> None:
+    _need(x.dim() == 2 and x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) % 8 == 0) and x.data_ptr() % 16 == 0,
+          "x must be [T, K] with contiguous rows that start on 16 bytes")
+
+
+def _check_w4(q: torch.Tensor, s: torch.Tensor, z: torch.Tensor | None, lead: tuple, n: int, k: int, dtype) -> int:
+    """Group size of the 4-bit weights ``[*lead, n, k]``."""
+    _need(q.dtype == torch.uint8 and q.shape == (*lead, n, k // 2) and k % 2 == 0 and q.is_contiguous(),
+          f"4-bit codes must be contiguous uint8 {[*lead, n, k // 2]}")
+    _need(s.dim() == q.dim() and s.shape[-1] > 0 and k % s.shape[-1] == 0, "scales must be [..., N, K / group]")
+    group = k // s.shape[-1]
+    _need(group in W4_GROUPS, f"group size must be one of {W4_GROUPS}, got {group}")
+    _need(s.dtype == dtype and s.shape == (*lead, n, k // group) and s.is_contiguous(),
+          f"scales must be contiguous {dtype} {[*lead, n, k // group]}")
+    _need(z is None or (z.dtype == torch.uint8 and z.shape == s.shape and z.is_contiguous()),
+          "zero points must be contiguous uint8 of the scales' shape")
+    return group
+
+
+def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x W^T`` for 4-bit weights with group scales and a few rows of ``x``.
+
+    ``x`` ``[T, K]`` bf16 or fp16; ``qweight`` uint8 ``[N, K / 2]`` (low nibble
+    = even k); ``scales`` ``[N, K / g]`` of x's type, g = 32, 64 or 128;
+    ``zeros`` uint8 ``[N, K / g]`` (None: 8).  ``w = (q - zero) * scale``, sums
+    in fp32, one rounding to x's type.  Right for any T, made for up to 32 rows
+    (a prompt's thousands belong on a dense product)."""
+    _check_here(x, qweight, scales, zeros)
+    _need(x.dtype in (torch.bfloat16, torch.float16), f"x must be bf16 or fp16, got {x.dtype}")
+    _check_rows(x)
+    t, k = x.shape
+    _need(qweight.dim() == 2 and qweight.shape[0] > 0 and k > 0, "qweight must be [N, K / 2]")
+    n = qweight.shape[0]
+    group = _check_w4(qweight, scales, zeros, (), n, k, x.dtype)
+    out = _rows_out(x, n, out)
+    if t:
+        call("hca_w4_linear", _p(out), out.stride(0), _p(x), x.stride(0), _p(qweight), _p(scales), _p(zeros), t, n, k,
+             group, int(x.dtype == torch.float16), _s())
+    return out
+
+
+def quantize_weight_w4(w: torch.Tensor, group: int = 128, asymmetric: bool = False, dtype=torch.bfloat16):
+    """Load-time 4-bit quant of ``w [..., N, K]`` for ``w4_linear`` and
+    ``MoEWeights``: ``(qweight uint8 [..., N, K / 2], scales [..., N, K / g] of
+    ``dtype``, zeros uint8 or None)``, nearest codes.  A one-off weight
+    transform, not a step of the forward pass."""
+    *lead, n, k = w.shape
+    _need(group in W4_GROUPS and k % group == 0, f"group size must be one of {W4_GROUPS} and divide K")
+    g = w.float().unflatten(-1, (k // group, group))
+    if asymmetric:
+        low, high = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)
+        scale = ((high - low) / 15).to(dtype)
+        step = torch.where(scale > 0, scale.float(), 1.0)
+        zero = torch.round(-low / step).clamp(0, 15)
+    else:
+        scale = (g.abs().amax(-1) / 7).to(dtype)
+        step = torch.where(scale > 0, scale.float(), 1.0)
+        zero = torch.full_like(step, 8.0)
+    codes = (torch.round(g / step.unsqueeze(-1)) + zero.unsqueeze(-1)).clamp(0, 15).to(torch.uint8).flatten(-2)
+    q = codes[..., 0::2] | (codes[..., 1::2] << 4)
+    return q.contiguous(), scale.contiguous(), zero.to(torch.uint8).contiguous() if asymmetric else None
+
+
+class MoEWeights(NamedTuple):
+    """Gated MLP weights of a stack of experts (or, without the leading
+    dimension, of a shared expert), in one of three formats by ``w13``'s type:
+
+    * bf16: ``w13 [E, 2 I, H]`` (gate rows over up rows), ``w2 [E, H, I]``;
+    * e4m3 with fp32 scales of 128 x 128 blocks, ``s13 [E, ceil(2 I / 128),
+      ceil(H / 128)]``, ``s2 [E, ceil(H / 128), ceil(I / 128)]``;
+    * uint8 4-bit codes ``[E, 2 I, H / 2]``, ``[E, H, I / 2]`` with bf16 group
+      scales and optional zero points, as ``w4_linear``."""
+
+    w13: torch.Tensor
+    w2: torch.Tensor
+    s13: torch.Tensor | None = None
+    s2: torch.Tensor | None = None
+    z13: torch.Tensor | None = None
+    z2: torch.Tensor | None = None
+
+
+_MOE_FORMATS = {torch.bfloat16: 0, FP8: 1, torch.uint8: 2}
+
+
+def _moe_weights(w: MoEWeights, lead: tuple, hidden: int) -> tuple[int, int, int]:
+    """``(format, group, inner)`` of checked weights."""
+    _check_here(*w)
+    fmt = _MOE_FORMATS.get(w.w13.dtype, -1)
+    _need(fmt >= 0 and w.w2.dtype == w.w13.dtype, "expert weights must be bf16, e4m3 or uint8 (4-bit codes), both alike")
+    rank = len(lead) + 2
+    _need(w.w13.dim() == rank and w.w2.dim() == rank and w.w13.shape[-2] % 2 == 0, f"expert weights must have {rank} dimensions")
+    inner = w.w13.shape[-2] // 2
+    if fmt == 2:
+        _need(w.s13 is not None and w.s2 is not None, "4-bit experts need scales")
+        group = _check_w4(w.w13, w.s13, w.z13, lead, 2 * inner, hidden, torch.bfloat16)
+        _need(_check_w4(w.w2, w.s2, w.z2, lead, hidden, inner, torch.bfloat16) == group, "w13 and w2 must have one group size")
+        return fmt, group, inner
+    _need(w.z13 is None and w.z2 is None, "only 4-bit experts have zero points")
+    for m, s, n, k in ((w.w13, w.s13, 2 * inner, hidden), (w.w2, w.s2, hidden, inner)):
+        _need(m.shape == (*lead, n, k) and m.is_contiguous(), f"expert weights must be contiguous {[*lead, n, k]}")
+        if fmt == 0:
+            _need(s is None, "bf16 experts have no scales")
+        else:
+            shape = (*lead, -(-n // 128), -(-k // 128))
+            _need(s is not None and s.dtype == torch.float32 and s.shape == shape and s.is_contiguous(),
+                  f"block scales must be contiguous fp32 {list(shape)}")
+    return fmt, 0, inner
+
+
+def _moe_args(x, experts: MoEWeights, shared: MoEWeights | None, token_mask):
+    """Checked ``(format, group, weight pointers, E, I, Is)``."""
+    _check_here(x, token_mask)
+    _need(x.dtype == torch.bfloat16, f"x must be bf16, got {x.dtype}")
+    _check_rows(x)
+    t, hidden = x.shape
+    _need(token_mask is None or (token_mask.dtype in (torch.bool, torch.uint8) and token_mask.shape == (t,)
+                                 and token_mask.is_contiguous()), f"token_mask must be contiguous bool [{t}]")
+    num = experts.w13.shape[0]
+    fmt, group, inner = _moe_weights(experts, (num,), hidden)
+    ptrs = [_p(m) for m in (experts.w13, experts.s13, experts.z13, experts.w2, experts.s2, experts.z2)]
+    shared_inner = 0
+    if shared is None:
+        ptrs += [None] * 6
+    else:
+        sfmt, sgroup, shared_inner = _moe_weights(shared, (), hidden)
+        _need((sfmt, sgroup) == (fmt, group), "the shared expert must have the experts' format")
+        ptrs += [_p(m) for m in (shared.w13, shared.s13, shared.z13, shared.w2, shared.s2, shared.z2)]
+    return fmt, group, ptrs, num, inner, shared_inner
+
+
+def _router_args(x, router_weight, router_bias, top_k: int, score: str):
+    _check_here(router_weight, router_bias)
+    _need(score in ("softmax", "sigmoid"), f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    _need(router_weight.dim() == 2 and router_weight.shape[1] == x.shape[1] and router_weight.is_contiguous()
+          and router_weight.dtype in (torch.bfloat16, torch.float32),
+          f"router_weight must be contiguous bf16 or fp32 [E, {x.shape[1]}]")
+    num = router_weight.shape[0]
+    _need(router_bias is None or (router_bias.dtype == torch.float32 and router_bias.shape == (num,)
+                                  and router_bias.is_contiguous()), f"router_bias must be contiguous fp32 [{num}]")
+    _need(1 <= top_k <= num, f"top_k must be 1 to {num}, got {top_k}")
+    return _p(router_weight), int(router_weight.dtype == torch.float32), _p(router_bias), int(score == "sigmoid")
+
+
+def moe_route(x: torch.Tensor, router_weight: torch.Tensor, top_k: int, *, score: str = "softmax",
+              router_bias: torch.Tensor | None = None, renormalize: bool = True, routed_scale: float = 1.0,
+              token_mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Router of a mixture-of-experts layer for a few tokens: ``(ids int32
+    [T, top_k], weights fp32 [T, top_k])``, largest score first.
+
+    ``x`` bf16 ``[T, H]``; ``router_weight`` ``[E, H]`` bf16 or fp32, products
+    in fp32.  Scores are ``softmax`` or ``sigmoid`` of the logits; experts are
+    chosen by score + ``router_bias`` (ties to the lower expert) and weighted by
+    the score alone, renormalised over the chosen ones if asked for, times
+    ``routed_scale``.  Rows that ``token_mask`` (bool ``[T]``) leaves out get
+    ids -1 and weights 0.  E <= 512, top_k <= 16, H a multiple of 32."""
+    _check_here(x, token_mask)
+    _need(x.dtype == torch.bfloat16, f"x must be bf16, got {x.dtype}")
+    _check_rows(x)
+    t, hidden = x.shape
+    wr, fp32, bias, sigmoid = _router_args(x, router_weight, router_bias, top_k, score)
+    _need(token_mask is None or (token_mask.dtype in (torch.bool, torch.uint8) and token_mask.shape == (t,)
+                                 and token_mask.is_contiguous()), f"token_mask must be contiguous bool [{t}]")
+    ids = torch.empty((t, top_k), dtype=torch.int32, device=x.device)
+    weights = torch.empty((t, top_k), dtype=torch.float32, device=x.device)
+    call("hca_moe_route", _p(ids), _p(weights), _p(x), x.stride(0), wr, fp32, bias, _p(token_mask), t,
+         router_weight.shape[0], hidden, top_k, sigmoid, int(renormalize), routed_scale, _s())
+    return ids, weights
+
+
+def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, experts: MoEWeights, *,
+                shared: MoEWeights | None = None, token_mask: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """Experts of a mixture-of-experts layer for a few tokens: ``y[t] = sum_j
+    weights[t, j] W2_e (silu(W1_e x_t) * (W3_e x_t))`` with ``e = ids[t, j]``,
+    plus the ``shared`` expert (weight 1).
+
+    ``ids`` int32 ``[T, top_k]`` (ids outside ``[0, E)`` are skipped, as for the
+    experts of another rank; an id may repeat), ``weights`` fp32 ``[T, top_k]``.
+    Each chosen expert's weights are read once for all its tokens (of 64 at a
+    time).  Rows that ``token_mask`` leaves out come out as 0 and choose
+    nothing.  The gated product is rounded to bf16 once, its weight included;
+    sums are fp32."""
+    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, experts, shared, token_mask)
+    _check_here(ids, weights)
+    t, hidden = x.shape
+    _need(ids.dtype == torch.int32 and ids.dim() == 2 and ids.shape[0] == t and ids.is_contiguous()
+          and weights.dtype == torch.float32 and weights.shape == ids.shape and weights.is_contiguous(),
+          f"ids must be contiguous int32 [{t}, top_k] and weights fp32 alike")
+    top_k = ids.shape[1]
+    out = _rows_out(x, hidden, out)
+    nbytes = lib().hca_moe_workspace_bytes(t, top_k, inner, shared_inner)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    call("hca_moe_experts", _p(out), out.stride(0), _p(x), x.stride(0), _p(ids), _p(weights), _p(token_mask), fmt, group,
+         *ptrs, t, num, hidden, inner, shared_inner, top_k, _p(ws), nbytes, _s())
+    return out
+
+
+def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts: MoEWeights, top_k: int, *, score: str = "softmax",
+               router_bias: torch.Tensor | None = None, renormalize: bool = True, routed_scale: float = 1.0,
+               shared: MoEWeights | None = None, token_mask: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """A whole mixture-of-experts layer for a few tokens (``moe_route`` then
+    ``moe_experts``) in one call; ``x`` and the result bf16 ``[T, H]``.  Its
+    scratch comes from the caching allocator on the current stream, so calls
+    on several streams do not meet."""
+    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, experts, shared, token_mask)
+    wr, fp32, bias, sigmoid = _router_args(x, router_weight, router_bias, top_k, score)
+    _need(router_weight.shape[0] == num, f"router_weight must have the {num} experts' rows")
+    t, hidden = x.shape
+    out = _rows_out(x, hidden, out)
+    nbytes = lib().hca_moe_workspace_bytes(t, top_k, inner, shared_inner)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    call("hca_moe_decode", _p(out), out.stride(0), _p(x), x.stride(0), wr, fp32, bias, sigmoid, int(renormalize),
+         routed_scale, _p(token_mask), fmt, group, *ptrs, t, num, hidden, inner, shared_inner, top_k, _p(ws), nbytes, _s())
+    return out
+
+
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def apply_logit_penalties(logits: torch.Tensor, token_ids: torch.Tensor | None = None,
+                          prompt_lens: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None, *,
+                          repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                          presence: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                          bias_values: torch.Tensor | None = None, allowed_bitmask: torch.Tensor | None = None,
+                          req_index: torch.Tensor | None = None) -> torch.Tensor:
+    """Biases, penalties for repeated tokens and a grammar mask on ``logits
+    [rows, V]`` (fp32, bf16 or fp16, contiguous rows), in place; returns them.
+
+    In this order: a biased token's ``x += bias``; a token of the prompt or the
+    answer ``x > 0 ? x / repetition : x * repetition``; one that the answer
+    holds n times ``x -= frequency * n + presence``; one that the mask does not
+    allow ``-inf``.  ``token_ids`` int32 ``[R, >= seq_len]``: row i's prompt is
+    ``[0, prompt_lens[i])`` and its answer ``[prompt_lens[i], seq_lens[i])`` of
+    request ``req_index[i]`` (int32; None: request i; outside ``[0, R)``: the
+    row is left alone), so a request's draft rows can share its tokens.
+    ``repetition``/``frequency``/``presence`` fp32 ``[R]``; ``bias_ids`` int32
+    and ``bias_values`` fp32 ``[R, M]`` (of an id listed twice the later
+    counts); ids outside ``[0, V)``, like -1, are skipped.  ``allowed_bitmask``
+    int32 ``[rows, ceil(V / 32)]``, bit ``v % 32`` of word ``v // 32``."""
+    _check_here(logits, token_ids, prompt_lens, seq_lens, repetition, frequency, presence, bias_ids, bias_values,
+                allowed_bitmask, req_index)
+    kind = _LOGIT_TYPES.get(logits.dtype, -1)
+    _need(kind >= 0, f"logits must be fp32, bf16 or fp16, got {logits.dtype}")
+    _need(logits.dim() == 2 and logits.shape[1] > 0 and (logits.shape[1] == 1 or logits.stride(1) == 1),
+          "logits must be [rows, V] with contiguous rows")
+    rows, vocab = logits.shape
+    tables = [t for t in (token_ids, repetition, frequency, presence, bias_ids, bias_values) if t is not None]
+    reqs = tables[0].shape[0] if tables else rows
+    for t in (repetition, frequency, presence):
+        _need(t is None or (t.dtype == torch.float32 and t.shape == (reqs,) and t.is_contiguous()),
+              f"penalties must be contiguous fp32 [{reqs}]")
+    if req_index is None:
+        _need(reqs == rows, f"{reqs} requests for {rows} rows need req_index")
+    else:
+        _need(req_index.dtype == torch.int32 and req_index.shape == (rows,) and req_index.is_contiguous(),
+              f"req_index must be contiguous int32 [{rows}]")
+    width = stride = 0
+    if token_ids is not None:
+        _need(token_ids.dtype == torch.int32 and token_ids.dim() == 2 and token_ids.shape[0] == reqs
+              and (token_ids.shape[1] <= 1 or token_ids.stride(1) == 1), f"token_ids must be int32 [{reqs}, L] with contiguous rows")
+        for t in (prompt_lens, seq_lens):
+            _need(t is not None and t.dtype == torch.int32 and t.shape == (rows,) and t.is_contiguous(),
+                  f"prompt_lens and seq_lens must be contiguous int32 [{rows}]")
+        width, stride = token_ids.shape[1], token_ids.stride(0)
+    bias_width = bias_stride = 0
+    _need((bias_ids is None) == (bias_values is None), "bias_ids and bias_values come together")
+    if bias_ids is not None:
+        _need(bias_ids.dtype == torch.int32 and bias_ids.dim() == 2 and bias_ids.shape[0] == reqs and bias_ids.is_contiguous()
+              and bias_values.dtype == torch.float32 and bias_values.shape == bias_ids.shape and bias_values.is_contiguous(),
+              f"bias_ids must be contiguous int32 [{reqs}, M] and bias_values fp32 alike")
+        bias_width = bias_stride = bias_ids.shape[1]
+    if allowed_bitmask is not None:
+        _need(allowed_bitmask.dtype == torch.int32 and allowed_bitmask.shape == (rows, -(-vocab // 32))
+              and allowed_bitmask.stride(1) == 1, f"allowed_bitmask must be int32 [{rows}, {-(-vocab // 32)}] with contiguous rows")
+    call("hca_logit_penalties", _p(logits), logits.stride(0), kind, _p(req_index), reqs, _p(token_ids), stride, width,
+         _p(prompt_lens), _p(seq_lens), _p(repetition), _p(frequency), _p(presence), _p(bias_ids), _p(bias_values),
+         bias_stride, bias_width, _p(allowed_bitmask), allowed_bitmask.stride(0) if allowed_bitmask is not None else 0, rows,
+         vocab, _s())
+    return logits
