@@ -460,11 +460,14 @@ int hca_w4_linear(void* out, int64_t out_stride, const void* x, int64_t x_stride
  * weights[t, j] = the score (without the bias), divided by the chosen ones'
  * sum with renormalize (0 where that sum is 0), times routed_scale.  Rows whose
  * token_mask byte is 0 get ids -1 and weights 0.  E <= 512, top_k <= 16 and
- * <= E, H a multiple of 32. */
+ * <= E, H a multiple of 32.  workspace as for the experts, of
+ * hca_moe_route_workspace_bytes(T, E) bytes. */
+int64_t hca_moe_route_workspace_bytes(int32_t num_tokens, int32_t num_experts);
 int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride, const void* router,
                   int32_t router_fp32, const float* router_bias, const uint8_t* token_mask,
                   int32_t num_tokens, int32_t num_experts, int32_t hidden, int32_t top_k,
-                  int32_t sigmoid, int32_t renormalize, float routed_scale, void* stream);
+                  int32_t sigmoid, int32_t renormalize, float routed_scale, void* workspace,
+                  int64_t workspace_bytes, void* stream);
 
 /* Weight formats of the expert matrices. */
 #define HCA_WEIGHT_BF16 0 /* [E, N, K] bf16 */
@@ -482,7 +485,8 @@ int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride,
  * everything else is summed in fp32.  Any T; passes of 64 tokens.
  * workspace: hca_moe_workspace_bytes(...) bytes, 16-byte aligned, not to be
  * shared by calls that are not ordered on one stream. */
-int64_t hca_moe_workspace_bytes(int32_t num_tokens, int32_t top_k, int32_t inner, int32_t shared_inner);
+int64_t hca_moe_workspace_bytes(int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                                int32_t inner, int32_t shared_inner);
 int hca_moe_experts(void* out, int64_t out_stride, const void* x, int64_t x_stride, const int32_t* ids,
                     const float* weights, const uint8_t* token_mask, int32_t format, int32_t group_size,
                     const void* w13, const void* w13_scale, const uint8_t* w13_zero, const void* w2,

@@ -56,20 +56,22 @@ def test_moe_statuses(route):
 
 def test_moe_workspace_is_for_one_pass_and_the_routing():
     f = _lib.lib().hca_moe_workspace_bytes
-    assert f(0, 8, 1024, 0) == 0 and f(1, 8, 0, 0) == 0
-    assert f(1, 8, 1024, 0) >= 8 * 1024 * 2 + 2 * 8 * 4
-    # the gated products of 64 tokens at most, however many tokens follow
-    assert f(1000, 8, 1024, 512) < 64 * (8 * 1024 + 512) * 2 + 2 * 1000 * 8 * 4 + 1024
+    assert f(0, 64, 8, 4096, 1024, 0) == 0 and f(1, 64, 8, 4096, 0, 0) == 0
+    assert f(1, 64, 8, 4096, 1024, 0) >= 8 * 1024 * 2 + 9 * 4096 * 4 + 64 * 4
+    # the intermediates of 64 tokens at most, however many tokens follow
+    assert f(1000, 64, 8, 4096, 1024, 512) < f(64, 64, 8, 4096, 1024, 512) + 1000 * 64 * 4 + 1024
 
 
 def test_route_statuses():
     f = _lib.lib().hca_moe_route
 
-    def status(ids=P, x=P, xs=128, router=P, t=2, e=8, h=128, k=2):
-        return f(ids, P, x, xs, router, 0, None, None, t, e, h, k, 0, 1, 1.0, None)
+    def status(ids=P, x=P, xs=128, router=P, t=2, e=8, h=128, k=2, ws=P, size=4096):
+        return f(ids, P, x, xs, router, 0, None, None, t, e, h, k, 0, 1, 1.0, ws, size, None)
 
     assert status(t=0) == 0
-    assert [status(ids=None), status(x=P + 8), status(xs=4), status(router=P + 8), status(k=9), status(e=0, k=0)] == [-1] * 6
+    assert [status(ids=None), status(x=P + 8), status(xs=4), status(router=P + 8), status(k=9), status(e=0, k=0),
+            status(ws=None), status(ws=P + 8)] == [-1] * 8
+    assert status(size=60) == -4
     assert [status(e=600), status(e=20, k=17), status(h=48)] == [-2] * 3
 
 

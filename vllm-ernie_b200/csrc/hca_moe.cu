@@ -1,30 +1,25 @@
-// The router of the few-token mixture-of-experts layer, and its C entries.
+// The router of the few-token mixture-of-experts layer, and the C entries.
 //
 //   l[t, e] = x_t . Wr_e;  p = softmax(l) or 1 / (1 + exp(-l))
 //   ids[t] = the top_k largest of p + bias, ties to the lower expert
 //   weights[t, j] = p[t, ids[t, j]] (/ their sum) * scale
 //
-// Latency-bound (E * hidden weights, a few MB at most): a cluster of eight
-// CTAs handles up to eight tokens.  Each CTA computes an eighth of the experts
-// for all of them, in 32-bit multiply-adds (a bf16 tensor product would make
-// near-ties of a 32-bit router fall differently), sends each token's logits to
-// the CTA of that token over distributed shared memory, and one warp there
-// picks the experts.  Nothing is counted in global memory, so nothing has to
-// be cleared between calls and calls on several streams do not meet.
+// The logits are latency-bound (experts * hidden weights, a few MB at most),
+// so they are spread over the whole GPU: a CTA computes two to four experts
+// for up to eight tokens, its warps splitting hidden.  Products and sums are
+// 32-bit multiply-adds: a bf16 tensor product would make near-ties of a 32-bit
+// router fall differently.  The choice itself is one warp's work a token, and
+// every CTA of the expert kernel makes it for itself.
 #include "hca_moe.cuh"
 #include "hca_stream.cuh"
 
 #include <algorithm>
-#include <cooperative_groups.h>
 
 namespace hca {
+
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr int kCluster = 8;
 constexpr int kWarps = 8;
-constexpr int kGroup = 4;  // experts of a warp at a time
 
 template <typename WT>
 __device__ __forceinline__ void load8(float (&v)[8], const WT* p) {
@@ -42,149 +37,101 @@ __device__ __forceinline__ void load8(float (&v)[8], const WT* p) {
   }
 }
 
-// Order-preserving key of a float; NaN below everything.
-__device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0;
-  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 orders as +0
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+// Sums of N values (a power of two up to 32) over the warp: each exchange adds
+// halves, so lane l ends with value `index` and N + 4 shuffles do for 5 N.
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N], int& index) {
+  const int lane = threadIdx.x & 31;
+  index = 0;
+  int n = N;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool upper = lane & o;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        if (i < n) {
+          const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      if (upper) index += n;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+  return v[0];
 }
 
-template <typename WT, int TB>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kWarps * 32)
-    moe_route_kernel(int32_t* ids, float* weights, const __nv_bfloat16* x, int64_t x_stride, const WT* router,
-                     const float* bias, const uint8_t* mask, int tokens, int experts, int hidden, int top_k,
-                     int sigmoid, int renormalize, float scale) {
-  __shared__ float part[kWarps][kMoeExperts / kCluster * TB];  // [warp][expert of the CTA * TB + token]
-  __shared__ float logits[kMoeExperts];                        // of this CTA's token
+// logits[t, e] for kExperts experts and TB tokens; block (0, 0) also clears
+// the words of `barriers`.
+template <typename WT, int TB, int kExperts>
+__global__ void __launch_bounds__(kWarps * 32)
+    moe_logits_kernel(float* logits, const __nv_bfloat16* x, int64_t x_stride, const WT* router, int tokens,
+                      int experts, int hidden, uint32_t* barriers, int num_barriers) {
+  __shared__ float part[kWarps][kExperts * TB];
   pdl_wait_and_release();
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank());
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < num_barriers; i += kWarps * 32) barriers[i] = 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x / kCluster * TB;
-  const int per = (experts + kCluster - 1) / kCluster;
-  const int e0 = rank * per, mine = max(0, min(per, experts - e0));
-
-  // warps split hidden in steps of 256 (8 values a lane)
-  const int steps = (hidden + 255) / 256;
-  const int s0 = steps * warp / kWarps, s1 = steps * (warp + 1) / kWarps;
-  for (int g = 0; g < mine; g += kGroup) {
-    float acc[kGroup][TB] = {};
-    for (int s = s0; s < s1; ++s) {
-      const int k = s * 256 + lane * 8;
-      if (k >= hidden) break;  // hidden is a multiple of 8
-      float wv[kGroup][8];
+  const int e0 = blockIdx.x * kExperts, t0 = blockIdx.y * TB;
+  float acc[kExperts * TB] = {};
+#pragma unroll 2
+  for (int k = (warp * 32 + lane) * 8; k < hidden; k += kWarps * 256) {  // hidden is a multiple of 8
+    float wv[kExperts][8];
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i)
-        load8(wv[i], router + static_cast<int64_t>(e0 + min(g + i, mine - 1)) * hidden + k);
+    for (int i = 0; i < kExperts; ++i) load8(wv[i], router + static_cast<int64_t>(min(e0 + i, experts - 1)) * hidden + k);
 #pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        float xv[8];
-        load8(xv, x + min(t0 + t, tokens - 1) * x_stride + k);
+    for (int t = 0; t < TB; ++t) {
+      float xv[8];
+      load8(xv, x + min(t0 + t, tokens - 1) * x_stride + k);
 #pragma unroll
-        for (int i = 0; i < kGroup; ++i)
+      for (int i = 0; i < kExperts; ++i)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) acc[i][t] = fmaf(xv[j], wv[i][j], acc[i][t]);
-      }
+        for (int j = 0; j < 8; ++j) acc[i * TB + t] = fmaf(xv[j], wv[i][j], acc[i * TB + t]);
     }
-#pragma unroll
-    for (int i = 0; i < kGroup; ++i)
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        const float v = warp_sum(acc[i][t]);
-        if (lane == 0 && g + i < mine) part[warp][(g + i) * TB + t] = v;
-      }
   }
+  int index;
+  const float v = warp_sums(acc, index);
+  part[warp][index] = v;
   __syncthreads();
-  for (int i = threadIdx.x; i < mine * TB; i += kWarps * 32) {
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += part[w][i];
-    *cluster.map_shared_rank(&logits[e0 + i / TB], i % TB) = v;
-  }
-  cluster.sync();  // every logit has arrived; no CTA touches another's memory after this
-
-  const int t = t0 + rank;
-  if (warp != 0 || rank >= TB || t >= tokens) return;
-  constexpr int kPer = kMoeExperts / 32;
-  float score[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = lane + 32 * j;
-    score[j] = e < experts ? logits[e] : -INFINITY;
-  }
-  if (sigmoid) {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) score[j] = 1.0f / (1.0f + expf(-score[j]));
-  } else {
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) m = fmaxf(m, score[j]);
-    m = warp_max(m);
+  for (int i = threadIdx.x; i < kExperts * TB; i += kWarps * 32) {
+    const int e = e0 + i / TB, t = t0 + i % TB;
+    if (e >= experts || t >= tokens) continue;
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (lane + 32 * j < experts) {
-        score[j] = expf(score[j] - m);
-        sum += score[j];
-      }
-    }
-    sum = warp_sum(sum);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) score[j] /= sum;
-  }
-  uint32_t key[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = lane + 32 * j;
-    // 0 is NaN's key, so real experts take key + 1 (no key is 2^32 - 1: that would be a NaN's) and taken or absent ones 0
-    key[j] = e < experts ? order_key(bias == nullptr ? score[j] : score[j] + bias[e]) + 1 : 0;
-  }
-  float chosen = 0.0f;  // lane j: the j-th choice's score
-  int chosen_id = -1;
-  for (int c = 0; c < top_k; ++c) {
-    uint32_t best = 0;
-    int at = 0;
-    float s = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (key[j] > best) best = key[j], at = j, s = score[j];
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : ~0u);
-    const float v = __shfl_sync(0xffffffffu, s, e & 31);
-    if (lane == static_cast<int>(e & 31)) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (j == static_cast<int>(e >> 5)) key[j] = 0;
-    }
-    if (lane == c) chosen = v, chosen_id = static_cast<int>(e);
-  }
-  float w = chosen;
-  if (renormalize) {
-    const float sum = warp_sum(lane < top_k ? chosen : 0.0f);
-    w = sum == 0.0f ? 0.0f : chosen / sum;  // every chosen score underflowed: no expert has weight
-  }
-  if (lane < top_k) {
-    const bool in = mask == nullptr || mask[t] != 0;
-    ids[t * top_k + lane] = in ? chosen_id : -1;
-    weights[t * top_k + lane] = in ? w * scale : 0.0f;
+    for (int w = 0; w < kWarps; ++w) sum += part[w][i];
+    logits[static_cast<int64_t>(t) * experts + e] = sum;
   }
 }
 
-template <typename WT, int TB>
-int launch_route(int32_t* ids, float* weights, const void* x, int64_t x_stride, const void* router, const float* bias,
-                 const uint8_t* mask, int tokens, int experts, int hidden, int top_k, int sigmoid, int renormalize,
-                 float scale, cudaStream_t s) {
-  return launch_pdl(moe_route_kernel<WT, TB>, dim3(cdiv(tokens, TB) * kCluster), dim3(kWarps * 32), 0, s, ids, weights,
-                    static_cast<const __nv_bfloat16*>(x), x_stride, static_cast<const WT*>(router), bias, mask, tokens,
-                    experts, hidden, top_k, sigmoid, renormalize, scale);
+template <typename WT, int TB, int kExperts>
+int launch_logits(float* logits, const void* x, int64_t x_stride, const void* router, int tokens, int experts,
+                  int hidden, uint32_t* barriers, int num_barriers, cudaStream_t s) {
+  return launch_pdl(moe_logits_kernel<WT, TB, kExperts>, dim3(cdiv(experts, kExperts), cdiv(tokens, TB)),
+                    dim3(kWarps * 32), 0, s, logits, static_cast<const __nv_bfloat16*>(x), x_stride,
+                    static_cast<const WT*>(router), tokens, experts, hidden, barriers, num_barriers);
 }
 
 template <typename WT, typename... A>
-int route_by_tokens(int tokens, A... a) {
-  if (tokens <= 1) return launch_route<WT, 1>(a...);
-  if (tokens <= 2) return launch_route<WT, 2>(a...);
-  if (tokens <= 4) return launch_route<WT, 4>(a...);
-  return launch_route<WT, 8>(a...);
+int logits_by_tokens(int tokens, A... a) {
+  // few tokens: more CTAs than reuse of x
+  if (tokens <= 1) return launch_logits<WT, 1, 2>(a...);
+  if (tokens <= 2) return launch_logits<WT, 2, 2>(a...);
+  if (tokens <= 4) return launch_logits<WT, 4, 2>(a...);
+  if (tokens <= 8) return launch_logits<WT, 8, 2>(a...);
+  return launch_logits<WT, 8, 4>(a...);
+}
+
+__global__ void __launch_bounds__(kWarps * 32)
+    moe_choose_kernel(int32_t* ids, float* weights, const float* logits, int tokens, MoeRouting r) {
+  pdl_wait_and_release();
+  const int t = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= tokens) return;
+  int id;
+  float weight;
+  choose_experts(logits + static_cast<int64_t>(t) * r.experts, r, t, id, weight);
+  if (lane < r.top_k) ids[static_cast<int64_t>(t) * r.top_k + lane] = id, weights[static_cast<int64_t>(t) * r.top_k + lane] = weight;
 }
 
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -192,55 +139,42 @@ bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) %
 int check_sizes(int tokens, int experts, int hidden, int top_k) {
   HCA_CHECK_ARG(tokens >= 0 && experts > 0 && hidden > 0 && top_k > 0 && top_k <= experts);
   if (experts > kMoeExperts || top_k > kMoeTopK || hidden % 32 != 0) return HCA_E_UNSUPPORTED;
+  HCA_CHECK_ARG(cdiv(tokens, 8) <= 65535);
   return HCA_OK;
 }
 
-int route(int32_t* ids, float* weights, const void* x, int64_t x_stride, const void* router, int router_fp32,
-          const float* bias, const uint8_t* mask, int tokens, int experts, int hidden, int top_k, int sigmoid,
-          int renormalize, float scale, cudaStream_t s) {
-  HCA_CHECK_ARG(ids && weights && x && router);
-  HCA_CHECK_ARG(aligned(x, 16) && x_stride % 8 == 0 && aligned(router, 16));
-  HCA_CHECK_ARG(cdiv(tokens, 8) <= 1 << 20);
-  return router_fp32 ? route_by_tokens<float>(tokens, ids, weights, x, x_stride, router, bias, mask, tokens, experts,
-                                              hidden, top_k, sigmoid, renormalize, scale, s)
-                     : route_by_tokens<__nv_bfloat16>(tokens, ids, weights, x, x_stride, router, bias, mask, tokens,
-                                                      experts, hidden, top_k, sigmoid, renormalize, scale, s);
+int check_rows(const void* x, int64_t x_stride) {
+  HCA_CHECK_ARG(x && aligned(x, 16) && x_stride % 8 == 0);
+  return HCA_OK;
+}
+
+int compute_logits(float* logits, const void* x, int64_t x_stride, const void* router, int router_fp32, int tokens,
+                   int experts, int hidden, uint32_t* barriers, int num_barriers, cudaStream_t s) {
+  return router_fp32
+             ? logits_by_tokens<float>(tokens, logits, x, x_stride, router, tokens, experts, hidden, barriers,
+                                       num_barriers, s)
+             : logits_by_tokens<__nv_bfloat16>(tokens, logits, x, x_stride, router, tokens, experts, hidden, barriers,
+                                               num_barriers, s);
 }
 
 int64_t align_up(int64_t v) { return (v + 255) / 256 * 256; }
+int64_t logit_bytes(int tokens, int experts) { return align_up(static_cast<int64_t>(tokens) * experts * 4); }
 
-int64_t h_bytes(int tokens, int top_k, int inner, int shared_inner) {
-  const int64_t t = std::min(tokens, kMoeTokens);
-  return align_up(t * (static_cast<int64_t>(top_k) * inner + shared_inner) * 2);
-}
-
-int experts_passes(void* out, int64_t out_stride, const void* x, int64_t x_stride, const int32_t* ids,
-                   const float* weights, const uint8_t* mask, int format, int group, const MoeWeights& w, int tokens,
-                   int experts, int hidden, int inner, int shared_inner, int top_k, __nv_bfloat16* h, cudaStream_t s) {
-  HCA_CHECK_ARG(out && x && ids && weights);
-  HCA_CHECK_ARG(aligned(x, 16) && x_stride % 8 == 0 && aligned(out, 2));
-  for (int t = 0; t < tokens; t += kMoeTokens) {
-    MoePass p;
-    p.x = static_cast<const __nv_bfloat16*>(x) + t * x_stride;
-    p.x_stride = x_stride;
-    p.ids = ids + static_cast<int64_t>(t) * top_k;
-    p.weights = weights + static_cast<int64_t>(t) * top_k;
-    p.mask = mask == nullptr ? nullptr : mask + t;
-    p.h = h;
-    p.out = static_cast<__nv_bfloat16*>(out) + t * out_stride;
-    p.out_stride = out_stride;
-    p.tokens = std::min(tokens - t, kMoeTokens);
-    p.top_k = top_k, p.experts = experts, p.hidden = hidden, p.inner = inner, p.shared_inner = shared_inner;
-    int rc = HCA_E_UNSUPPORTED;
-    if (format == HCA_WEIGHT_BF16) rc = moe_experts_pass<kWBf16>(p, w, s);
-    else if (format == HCA_WEIGHT_FP8) rc = moe_experts_pass<kWFp8>(p, w, s);
-    else if (group == 32) rc = moe_experts_pass<kW4G32>(p, w, s);
-    else if (group == 64) rc = moe_experts_pass<kW4G64>(p, w, s);
-    else if (group == 128) rc = moe_experts_pass<kW4G128>(p, w, s);
-    if (rc != HCA_OK) return rc;
+// Scratch of a call: gated products and the pairs' shares of y of one pass,
+// a barrier word a pass, and the logits.
+struct Scratch {
+  int64_t h, part, barriers, logits, total;
+  int passes;
+  Scratch(int tokens, int experts, int top_k, int hidden, int inner, int shared_inner) {
+    const int64_t t = std::min(tokens, kMoeTokens);
+    passes = cdiv(tokens, kMoeTokens);
+    h = 0;
+    part = align_up(t * (static_cast<int64_t>(top_k) * inner + shared_inner) * 2);
+    barriers = part + align_up(t * (top_k + 1) * hidden * 4);
+    logits = barriers + align_up(4ll * passes);
+    total = logits + logit_bytes(tokens, experts);
   }
-  return HCA_OK;
-}
+};
 
 int check_matrix(const MoeMatrix& m, int format) {
   HCA_CHECK_ARG(m.data && aligned(m.data, 16));
@@ -263,6 +197,42 @@ int check_weights(const MoeWeights& w, int format, int group, int hidden, int in
   return rc;
 }
 
+// One layer's passes over 64 tokens each; either logits or ids and weights.
+int experts_passes(void* out, int64_t out_stride, const void* x, int64_t x_stride, const float* logits,
+                   const int32_t* ids, const float* weights, const MoeRouting& routing, int format, int group,
+                   const MoeWeights& w, int tokens, int hidden, int inner, int shared_inner, uint8_t* workspace,
+                   const Scratch& at, cudaStream_t s) {
+  int32_t* error = device_error_word();
+  if (error == nullptr) return HCA_E_CUDA;
+  for (int i = 0; i < at.passes; ++i) {
+    const int t = i * kMoeTokens;
+    MoePass p;
+    p.x = static_cast<const __nv_bfloat16*>(x) + t * x_stride;
+    p.x_stride = x_stride;
+    p.logits = logits == nullptr ? nullptr : logits + static_cast<int64_t>(t) * routing.experts;
+    p.ids = ids == nullptr ? nullptr : ids + static_cast<int64_t>(t) * routing.top_k;
+    p.weights = weights == nullptr ? nullptr : weights + static_cast<int64_t>(t) * routing.top_k;
+    p.h = reinterpret_cast<__nv_bfloat16*>(workspace + at.h);
+    p.part = reinterpret_cast<float*>(workspace + at.part);
+    p.barrier = reinterpret_cast<uint32_t*>(workspace + at.barriers) + i;
+    p.error = error;
+    p.out = static_cast<__nv_bfloat16*>(out) + t * out_stride;
+    p.out_stride = out_stride;
+    p.routing = routing;
+    if (p.routing.mask != nullptr) p.routing.mask += t;
+    p.tokens = std::min(tokens - t, kMoeTokens);
+    p.hidden = hidden, p.inner = inner, p.shared_inner = shared_inner;
+    int rc = HCA_E_UNSUPPORTED;
+    if (format == HCA_WEIGHT_BF16) rc = moe_experts_pass<kWBf16>(p, w, s);
+    else if (format == HCA_WEIGHT_FP8) rc = moe_experts_pass<kWFp8>(p, w, s);
+    else if (group == 32) rc = moe_experts_pass<kW4G32>(p, w, s);
+    else if (group == 64) rc = moe_experts_pass<kW4G64>(p, w, s);
+    else if (group == 128) rc = moe_experts_pass<kW4G128>(p, w, s);
+    if (rc != HCA_OK) return rc;
+  }
+  return HCA_OK;
+}
+
 MoeMatrix matrix(const void* data, const void* scale, const uint8_t* zero) {
   return {static_cast<const uint8_t*>(data), scale, zero};
 }
@@ -270,21 +240,36 @@ MoeMatrix matrix(const void* data, const void* scale, const uint8_t* zero) {
 }  // namespace
 }  // namespace hca
 
+extern "C" int64_t hca_moe_route_workspace_bytes(int32_t num_tokens, int32_t num_experts) {
+  return num_tokens <= 0 || num_experts <= 0 ? 0 : hca::logit_bytes(num_tokens, num_experts);
+}
+
 extern "C" int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride, const void* router,
                              int32_t router_fp32, const float* router_bias, const uint8_t* token_mask,
                              int32_t num_tokens, int32_t num_experts, int32_t hidden, int32_t top_k, int32_t sigmoid,
-                             int32_t renormalize, float routed_scale, void* stream) {
+                             int32_t renormalize, float routed_scale, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
   using namespace hca;
-  const int rc = check_sizes(num_tokens, num_experts, hidden, top_k);
+  int rc = check_sizes(num_tokens, num_experts, hidden, top_k);
   if (rc != HCA_OK || num_tokens == 0) return rc;
-  return route(ids, weights, x, x_stride, router, router_fp32, router_bias, token_mask, num_tokens, num_experts,
-               hidden, top_k, sigmoid, renormalize, routed_scale, as_stream(stream));
+  rc = check_rows(x, x_stride);
+  if (rc != HCA_OK) return rc;
+  HCA_CHECK_ARG(ids && weights && router && aligned(router, 16));
+  if (workspace_bytes < logit_bytes(num_tokens, num_experts)) return HCA_E_WORKSPACE;
+  HCA_CHECK_ARG(workspace && aligned(workspace, 16));
+  cudaStream_t s = as_stream(stream);
+  float* logits = static_cast<float*>(workspace);
+  rc = compute_logits(logits, x, x_stride, router, router_fp32, num_tokens, num_experts, hidden, nullptr, 0, s);
+  if (rc != HCA_OK) return rc;
+  const MoeRouting r{router_bias, token_mask, num_experts, top_k, sigmoid, renormalize, routed_scale};
+  return launch_pdl(moe_choose_kernel, dim3(cdiv(num_tokens, kWarps)), dim3(kWarps * 32), 0, s, ids, weights, logits,
+                    num_tokens, r);
 }
 
-extern "C" int64_t hca_moe_workspace_bytes(int32_t num_tokens, int32_t top_k, int32_t inner, int32_t shared_inner) {
-  if (num_tokens <= 0 || top_k <= 0 || inner <= 0 || shared_inner < 0) return 0;
-  return hca::h_bytes(num_tokens, top_k, inner, shared_inner) +
-         2 * hca::align_up(static_cast<int64_t>(num_tokens) * top_k * 4);
+extern "C" int64_t hca_moe_workspace_bytes(int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
+                                           int32_t inner, int32_t shared_inner) {
+  if (num_tokens <= 0 || num_experts <= 0 || top_k <= 0 || hidden <= 0 || inner <= 0 || shared_inner < 0) return 0;
+  return hca::Scratch(num_tokens, num_experts, top_k, hidden, inner, shared_inner).total;
 }
 
 extern "C" int hca_moe_experts(void* out, int64_t out_stride, const void* x, int64_t x_stride, const int32_t* ids,
@@ -301,13 +286,21 @@ extern "C" int hca_moe_experts(void* out, int64_t out_stride, const void* x, int
   // ids may come from elsewhere and repeat, so top_k may exceed the experts of this rank
   HCA_CHECK_ARG(num_tokens >= 0 && num_experts > 0 && hidden > 0 && top_k > 0);
   if (num_experts > kMoeExperts || top_k > kMoeTopK || hidden % 32 != 0) return HCA_E_UNSUPPORTED;
-  const int rc = check_weights(w, format, group_size, hidden, inner, shared_inner);
+  int rc = check_weights(w, format, group_size, hidden, inner, shared_inner);
   if (rc != HCA_OK || num_tokens == 0) return rc;
-  if (workspace_bytes < h_bytes(num_tokens, top_k, inner, shared_inner)) return HCA_E_WORKSPACE;
+  const Scratch at(num_tokens, num_experts, top_k, hidden, inner, shared_inner);
+  if (workspace_bytes < at.total) return HCA_E_WORKSPACE;
   HCA_CHECK_ARG(workspace && aligned(workspace, 16));
-  return experts_passes(out, out_stride, x, x_stride, ids, weights, token_mask, format, group_size, w, num_tokens,
-                        num_experts, hidden, inner, shared_inner, top_k, static_cast<__nv_bfloat16*>(workspace),
-                        as_stream(stream));
+  HCA_CHECK_ARG(out && aligned(out, 2) && ids && weights);
+  rc = check_rows(x, x_stride);
+  if (rc != HCA_OK) return rc;
+  cudaStream_t s = as_stream(stream);
+  uint8_t* scratch = static_cast<uint8_t*>(workspace);
+  rc = cuda_status(cudaMemsetAsync(scratch + at.barriers, 0, 4ll * at.passes, s));
+  if (rc != HCA_OK) return rc;
+  const MoeRouting r{nullptr, token_mask, num_experts, top_k, 0, 0, 1.0f};
+  return experts_passes(out, out_stride, x, x_stride, nullptr, ids, weights, r, format, group_size, w, num_tokens,
+                        hidden, inner, shared_inner, scratch, at, s);
 }
 
 extern "C" int hca_moe_decode(void* out, int64_t out_stride, const void* x, int64_t x_stride, const void* router,
@@ -325,18 +318,19 @@ extern "C" int hca_moe_decode(void* out, int64_t out_stride, const void* x, int6
   int rc = check_sizes(num_tokens, num_experts, hidden, top_k);
   if (rc == HCA_OK) rc = check_weights(w, format, group_size, hidden, inner, shared_inner);
   if (rc != HCA_OK || num_tokens == 0) return rc;
-  if (workspace_bytes < hca_moe_workspace_bytes(num_tokens, top_k, inner, shared_inner)) return HCA_E_WORKSPACE;
+  const Scratch at(num_tokens, num_experts, top_k, hidden, inner, shared_inner);
+  if (workspace_bytes < at.total) return HCA_E_WORKSPACE;
   HCA_CHECK_ARG(workspace && aligned(workspace, 16));
-  HCA_CHECK_ARG(out && aligned(out, 2));
-  uint8_t* at = static_cast<uint8_t*>(workspace);
-  __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(at);
-  at += h_bytes(num_tokens, top_k, inner, shared_inner);
-  int32_t* ids = reinterpret_cast<int32_t*>(at);
-  at += align_up(static_cast<int64_t>(num_tokens) * top_k * 4);
-  float* weights = reinterpret_cast<float*>(at);
-  rc = route(ids, weights, x, x_stride, router, router_fp32, router_bias, token_mask, num_tokens, num_experts, hidden,
-             top_k, sigmoid, renormalize, routed_scale, as_stream(stream));
+  HCA_CHECK_ARG(out && aligned(out, 2) && router && aligned(router, 16));
+  rc = check_rows(x, x_stride);
   if (rc != HCA_OK) return rc;
-  return experts_passes(out, out_stride, x, x_stride, ids, weights, token_mask, format, group_size, w, num_tokens,
-                        num_experts, hidden, inner, shared_inner, top_k, h, as_stream(stream));
+  cudaStream_t s = as_stream(stream);
+  uint8_t* scratch = static_cast<uint8_t*>(workspace);
+  float* logits = reinterpret_cast<float*>(scratch + at.logits);
+  rc = compute_logits(logits, x, x_stride, router, router_fp32, num_tokens, num_experts, hidden,
+                      reinterpret_cast<uint32_t*>(scratch + at.barriers), at.passes, s);
+  if (rc != HCA_OK) return rc;
+  const MoeRouting r{router_bias, token_mask, num_experts, top_k, sigmoid, renormalize, routed_scale};
+  return experts_passes(out, out_stride, x, x_stride, logits, nullptr, nullptr, r, format, group_size, w, num_tokens,
+                        hidden, inner, shared_inner, scratch, at, s);
 }

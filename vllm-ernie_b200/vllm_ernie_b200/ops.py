@@ -730,8 +730,11 @@ def moe_route(x: torch.Tensor, router_weight: torch.Tensor, top_k: int, *, score
                                  and token_mask.is_contiguous()), f"token_mask must be contiguous bool [{t}]")
     ids = torch.empty((t, top_k), dtype=torch.int32, device=x.device)
     weights = torch.empty((t, top_k), dtype=torch.float32, device=x.device)
-    call("hca_moe_route", _p(ids), _p(weights), _p(x), x.stride(0), wr, fp32, bias, _p(token_mask), t,
-         router_weight.shape[0], hidden, top_k, sigmoid, int(renormalize), routed_scale, _s())
+    num = router_weight.shape[0]
+    nbytes = lib().hca_moe_route_workspace_bytes(t, num)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    call("hca_moe_route", _p(ids), _p(weights), _p(x), x.stride(0), wr, fp32, bias, _p(token_mask), t, num, hidden, top_k,
+         sigmoid, int(renormalize), routed_scale, _p(ws), nbytes, _s())
     return ids, weights
 
 
@@ -756,7 +759,7 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
           f"ids must be contiguous int32 [{t}, top_k] and weights fp32 alike")
     top_k = ids.shape[1]
     out = _rows_out(x, hidden, out)
-    nbytes = lib().hca_moe_workspace_bytes(t, top_k, inner, shared_inner)
+    nbytes = lib().hca_moe_workspace_bytes(t, num, top_k, hidden, inner, shared_inner)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     call("hca_moe_experts", _p(out), out.stride(0), _p(x), x.stride(0), _p(ids), _p(weights), _p(token_mask), fmt, group,
          *ptrs, t, num, hidden, inner, shared_inner, top_k, _p(ws), nbytes, _s())
@@ -776,7 +779,7 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts: MoEWeights
     _need(router_weight.shape[0] == num, f"router_weight must have the {num} experts' rows")
     t, hidden = x.shape
     out = _rows_out(x, hidden, out)
-    nbytes = lib().hca_moe_workspace_bytes(t, top_k, inner, shared_inner)
+    nbytes = lib().hca_moe_workspace_bytes(t, num, top_k, hidden, inner, shared_inner)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     call("hca_moe_decode", _p(out), out.stride(0), _p(x), x.stride(0), wr, fp32, bias, sigmoid, int(renormalize),
          routed_scale, _p(token_mask), fmt, group, *ptrs, t, num, hidden, inner, shared_inner, top_k, _p(ws), nbytes, _s())
