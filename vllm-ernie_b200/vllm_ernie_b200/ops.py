@@ -541,47 +541,64 @@ def quantize_weight_block_fp8(w: torch.Tensor, block: int = 128):
 # ---------------------------------------------------------------------------
 
 W4_GROUPS = (32, 64, 128)
+_BF16, _FP16, _FP32, _U8, _I32 = torch.bfloat16, torch.float16, torch.float32, torch.uint8, torch.int32
 
 
-def _need(cond: bool, what: str) -> None:
-    if not cond:
-        raise ValueError(what)
+def _refuse(what: str):
+    raise ValueError(what)
 
 
-def _check_here(*ts: torch.Tensor | None) -> None:
-    """Every tensor on the current device, whose current stream is used."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+# These operators take microseconds on the GPU, so their checks read each
+# attribute once and put no message together before it is needed.
+
+
+def _device_of(x: torch.Tensor, *ts: torch.Tensor | None) -> int:
+    """The device of all the tensors, which has to be the current one."""
+    dev = x.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        _refuse("libhca_b200 ops take CUDA tensors of the current device")
     for t in ts:
-        if t is not None and (not t.is_cuda or t.get_device() != here):
-            raise ValueError("libhca_b200 ops take CUDA tensors of the current device")
+        if t is not None and t.get_device() != dev:
+            _refuse("libhca_b200 ops take CUDA tensors of the current device")
+    return dev
 
 
-def _rows_out(x: torch.Tensor, n: int, out: torch.Tensor | None) -> torch.Tensor:
+def _stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _rows_out(x: torch.Tensor, dev: int, t: int, n: int, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        return torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
-    _check_here(out)
-    _need(out.shape == (x.shape[0], n) and out.dtype == x.dtype and (n == 1 or out.stride(1) == 1),
-          f"out must be {x.dtype} [{x.shape[0]}, {n}] with contiguous rows")
+        return x.new_empty((t, n))
+    if (out.get_device() != dev or out.dtype is not x.dtype or out.shape != (t, n) or (n > 1 and out.stride(1) != 1)):
+        _refuse(f"out must be {x.dtype} [{t}, {n}] with contiguous rows, on x's device")
     return out
 
 
-def _check_rows(x: torch.Tensor) -> None:
-    _need(x.dim() == 2 and x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) % 8 == 0) and x.data_ptr() % 16 == 0,
-          "x must be [T, K] with contiguous rows that start on 16 bytes")
+def _check_rows(x: torch.Tensor) -> tuple[int, int, int, int]:
+    """``(T, K, row stride, address)`` of a matrix whose rows start on 16 bytes."""
+    if x.dim() != 2:
+        _refuse("x must be [T, K]")
+    t, k = x.shape
+    stride, inner = x.stride()
+    at = x.data_ptr()
+    if (k > 1 and inner != 1) or (t > 1 and stride % 8) or at % 16:
+        _refuse("x must have contiguous rows that start on 16 bytes")
+    return t, k, stride if t > 1 else k + -k % 8, at
 
 
-def _check_w4(q: torch.Tensor, s: torch.Tensor, z: torch.Tensor | None, lead: tuple, n: int, k: int, dtype) -> int:
+def _check_w4(q, s, z, lead: tuple, n: int, k: int, dtype) -> int:
     """Group size of the 4-bit weights ``[*lead, n, k]``."""
-    _need(q.dtype == torch.uint8 and q.shape == (*lead, n, k // 2) and k % 2 == 0 and q.is_contiguous(),
-          f"4-bit codes must be contiguous uint8 {[*lead, n, k // 2]}")
-    _need(s.dim() == q.dim() and s.shape[-1] > 0 and k % s.shape[-1] == 0, "scales must be [..., N, K / group]")
-    group = k // s.shape[-1]
-    _need(group in W4_GROUPS, f"group size must be one of {W4_GROUPS}, got {group}")
-    _need(s.dtype == dtype and s.shape == (*lead, n, k // group) and s.is_contiguous(),
-          f"scales must be contiguous {dtype} {[*lead, n, k // group]}")
-    _need(z is None or (z.dtype == torch.uint8 and z.shape == s.shape and z.is_contiguous()),
-          "zero points must be contiguous uint8 of the scales' shape")
-    return group
+    if q.dtype is not _U8 or k % 2 or q.shape != (*lead, n, k // 2) or not q.is_contiguous():
+        _refuse(f"4-bit codes must be contiguous uint8 {[*lead, n, k // 2]}")
+    shape = s.shape
+    if len(shape) != len(lead) + 2 or shape[-1] == 0 or k % shape[-1] or k // shape[-1] not in W4_GROUPS:
+        _refuse(f"scales must be [..., N, K / group] for a group of {W4_GROUPS}")
+    if s.dtype is not dtype or shape[:-1] != (*lead, n) or not s.is_contiguous():
+        _refuse(f"scales must be contiguous {dtype} {[*lead, n, shape[-1]]}")
+    if z is not None and (z.dtype is not _U8 or z.shape != shape or not z.is_contiguous()):
+        _refuse("zero points must be contiguous uint8 of the scales' shape")
+    return k // shape[-1]
 
 
 def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
@@ -591,19 +608,22 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
     ``x`` ``[T, K]`` bf16 or fp16; ``qweight`` uint8 ``[N, K / 2]`` (low nibble
     = even k); ``scales`` ``[N, K / g]`` of x's type, g = 32, 64 or 128;
     ``zeros`` uint8 ``[N, K / g]`` (None: 8).  ``w = (q - zero) * scale``, sums
-    in fp32, one rounding to x's type.  Right for any T, made for up to 32 rows
-    (a prompt's thousands belong on a dense product)."""
-    _check_here(x, qweight, scales, zeros)
-    _need(x.dtype in (torch.bfloat16, torch.float16), f"x must be bf16 or fp16, got {x.dtype}")
-    _check_rows(x)
-    t, k = x.shape
-    _need(qweight.dim() == 2 and qweight.shape[0] > 0 and k > 0, "qweight must be [N, K / 2]")
+    in fp32, one rounding to x's type.  Right for any T, made for up to 16 rows
+    (each 16 more read the weights again; a prompt's thousands belong on a dense
+    product)."""
+    dev = _device_of(x, qweight, scales, zeros)
+    dtype = x.dtype
+    if dtype is not _BF16 and dtype is not _FP16:
+        _refuse(f"x must be bf16 or fp16, got {dtype}")
+    t, k, stride, at = _check_rows(x)
+    if qweight.dim() != 2 or qweight.shape[0] == 0 or k == 0:
+        _refuse("qweight must be [N, K / 2]")
     n = qweight.shape[0]
-    group = _check_w4(qweight, scales, zeros, (), n, k, x.dtype)
-    out = _rows_out(x, n, out)
+    group = _check_w4(qweight, scales, zeros, (), n, k, dtype)
+    out = _rows_out(x, dev, t, n, out)
     if t:
-        call("hca_w4_linear", _p(out), out.stride(0), _p(x), x.stride(0), _p(qweight), _p(scales), _p(zeros), t, n, k,
-             group, int(x.dtype == torch.float16), _s())
+        call("hca_w4_linear", out.data_ptr(), out.stride(0), at, stride, qweight.data_ptr(), scales.data_ptr(), _p(zeros), t,
+             n, k, group, dtype is _FP16, _stream(dev))
     return out
 
 
@@ -613,7 +633,8 @@ def quantize_weight_w4(w: torch.Tensor, group: int = 128, asymmetric: bool = Fal
     ``dtype``, zeros uint8 or None)``, nearest codes.  A one-off weight
     transform, not a step of the forward pass."""
     *lead, n, k = w.shape
-    _need(group in W4_GROUPS and k % group == 0, f"group size must be one of {W4_GROUPS} and divide K")
+    if group not in W4_GROUPS or k % group:
+        _refuse(f"group size must be one of {W4_GROUPS} and divide K")
     g = w.float().unflatten(-1, (k // group, group))
     if asymmetric:
         low, high = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)
@@ -650,63 +671,78 @@ class MoEWeights(NamedTuple):
 _MOE_FORMATS = {torch.bfloat16: 0, FP8: 1, torch.uint8: 2}
 
 
-def _moe_weights(w: MoEWeights, lead: tuple, hidden: int) -> tuple[int, int, int]:
-    """``(format, group, inner)`` of checked weights."""
-    _check_here(*w)
-    fmt = _MOE_FORMATS.get(w.w13.dtype, -1)
-    _need(fmt >= 0 and w.w2.dtype == w.w13.dtype, "expert weights must be bf16, e4m3 or uint8 (4-bit codes), both alike")
-    rank = len(lead) + 2
-    _need(w.w13.dim() == rank and w.w2.dim() == rank and w.w13.shape[-2] % 2 == 0, f"expert weights must have {rank} dimensions")
-    inner = w.w13.shape[-2] // 2
+def _moe_weights(w: MoEWeights, lead: tuple, hidden: int, dev: int) -> tuple[int, int, int, tuple]:
+    """``(format, group, inner, addresses)`` of checked weights."""
+    w13, w2, s13, s2, z13, z2 = w
+    for m in w:
+        if m is not None and m.get_device() != dev:
+            _refuse("expert weights must be on x's device")
+    fmt = _MOE_FORMATS.get(w13.dtype, -1)
+    if fmt < 0 or w2.dtype is not w13.dtype:
+        _refuse("expert weights must be bf16, e4m3 or uint8 (4-bit codes), both alike")
+    shape = w13.shape
+    if len(shape) != len(lead) + 2 or shape[-2] % 2 or shape[-2] == 0:
+        _refuse(f"w13 must be {[*lead, '2 I', 'H']}")
+    inner = shape[-2] // 2
     if fmt == 2:
-        _need(w.s13 is not None and w.s2 is not None, "4-bit experts need scales")
-        group = _check_w4(w.w13, w.s13, w.z13, lead, 2 * inner, hidden, torch.bfloat16)
-        _need(_check_w4(w.w2, w.s2, w.z2, lead, hidden, inner, torch.bfloat16) == group, "w13 and w2 must have one group size")
-        return fmt, group, inner
-    _need(w.z13 is None and w.z2 is None, "only 4-bit experts have zero points")
-    for m, s, n, k in ((w.w13, w.s13, 2 * inner, hidden), (w.w2, w.s2, hidden, inner)):
-        _need(m.shape == (*lead, n, k) and m.is_contiguous(), f"expert weights must be contiguous {[*lead, n, k]}")
-        if fmt == 0:
-            _need(s is None, "bf16 experts have no scales")
-        else:
-            shape = (*lead, -(-n // 128), -(-k // 128))
-            _need(s is not None and s.dtype == torch.float32 and s.shape == shape and s.is_contiguous(),
-                  f"block scales must be contiguous fp32 {list(shape)}")
-    return fmt, 0, inner
-
-
-def _moe_args(x, experts: MoEWeights, shared: MoEWeights | None, token_mask):
-    """Checked ``(format, group, weight pointers, E, I, Is)``."""
-    _check_here(x, token_mask)
-    _need(x.dtype == torch.bfloat16, f"x must be bf16, got {x.dtype}")
-    _check_rows(x)
-    t, hidden = x.shape
-    _need(token_mask is None or (token_mask.dtype in (torch.bool, torch.uint8) and token_mask.shape == (t,)
-                                 and token_mask.is_contiguous()), f"token_mask must be contiguous bool [{t}]")
-    num = experts.w13.shape[0]
-    fmt, group, inner = _moe_weights(experts, (num,), hidden)
-    ptrs = [_p(m) for m in (experts.w13, experts.s13, experts.z13, experts.w2, experts.s2, experts.z2)]
-    shared_inner = 0
-    if shared is None:
-        ptrs += [None] * 6
+        if s13 is None or s2 is None:
+            _refuse("4-bit experts need scales")
+        group = _check_w4(w13, s13, z13, lead, 2 * inner, hidden, _BF16)
+        if _check_w4(w2, s2, z2, lead, hidden, inner, _BF16) != group:
+            _refuse("w13 and w2 must have one group size")
+        return fmt, group, inner, (w13.data_ptr(), s13.data_ptr(), _p(z13), w2.data_ptr(), s2.data_ptr(), _p(z2))
+    if z13 is not None or z2 is not None:
+        _refuse("only 4-bit experts have zero points")
+    if shape != (*lead, 2 * inner, hidden) or w2.shape != (*lead, hidden, inner) or not (w13.is_contiguous() and w2.is_contiguous()):
+        _refuse(f"expert weights must be contiguous {[*lead, 2 * inner, hidden]} and {[*lead, hidden, inner]}")
+    if fmt == 0:
+        if s13 is not None or s2 is not None:
+            _refuse("bf16 experts have no scales")
     else:
-        sfmt, sgroup, shared_inner = _moe_weights(shared, (), hidden)
-        _need((sfmt, sgroup) == (fmt, group), "the shared expert must have the experts' format")
-        ptrs += [_p(m) for m in (shared.w13, shared.s13, shared.z13, shared.w2, shared.s2, shared.z2)]
-    return fmt, group, ptrs, num, inner, shared_inner
+        for s, n, k in ((s13, 2 * inner, hidden), (s2, hidden, inner)):
+            if s is None or s.dtype is not _FP32 or s.shape != (*lead, -(-n // 128), -(-k // 128)) or not s.is_contiguous():
+                _refuse(f"block scales must be contiguous fp32 {[*lead, -(-n // 128), -(-k // 128)]}")
+    return fmt, 0, inner, (w13.data_ptr(), _p(s13), None, w2.data_ptr(), _p(s2), None)
 
 
-def _router_args(x, router_weight, router_bias, top_k: int, score: str):
-    _check_here(router_weight, router_bias)
-    _need(score in ("softmax", "sigmoid"), f"score must be 'softmax' or 'sigmoid', got {score!r}")
-    _need(router_weight.dim() == 2 and router_weight.shape[1] == x.shape[1] and router_weight.is_contiguous()
-          and router_weight.dtype in (torch.bfloat16, torch.float32),
-          f"router_weight must be contiguous bf16 or fp32 [E, {x.shape[1]}]")
+def _moe_args(x, dev: int, hidden: int, experts: MoEWeights, shared: MoEWeights | None):
+    """Checked ``(format, group, weight addresses, E, I, Is)``."""
+    num = experts[0].shape[0]
+    fmt, group, inner, ptrs = _moe_weights(experts, (num,), hidden, dev)
+    if shared is None:
+        return fmt, group, ptrs + (None,) * 6, num, inner, 0
+    sfmt, sgroup, shared_inner, more = _moe_weights(shared, (), hidden, dev)
+    if sfmt != fmt or sgroup != group:
+        _refuse("the shared expert must have the experts' format")
+    return fmt, group, ptrs + more, num, inner, shared_inner
+
+
+def _moe_rows(x, token_mask, *ts) -> tuple[int, int, int, int, int]:
+    """Checked ``(device, T, H, row stride, address)`` of the layer's input."""
+    dev = _device_of(x, token_mask, *ts)
+    if x.dtype is not _BF16:
+        _refuse(f"x must be bf16, got {x.dtype}")
+    t, hidden, stride, at = _check_rows(x)
+    if token_mask is not None and (token_mask.dtype not in (torch.bool, _U8) or token_mask.shape != (t,)
+                                   or not token_mask.is_contiguous()):
+        _refuse(f"token_mask must be contiguous bool [{t}]")
+    return dev, t, hidden, stride, at
+
+
+def _router_args(hidden: int, router_weight, router_bias, top_k: int, score: str) -> tuple[int, int, int, int | None, int]:
+    """Checked ``(E, address, is fp32, bias address, is sigmoid)``."""
+    if score != "softmax" and score != "sigmoid":
+        _refuse(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    dtype = router_weight.dtype
+    if (router_weight.dim() != 2 or router_weight.shape[1] != hidden or not router_weight.is_contiguous()
+            or (dtype is not _BF16 and dtype is not _FP32)):
+        _refuse(f"router_weight must be contiguous bf16 or fp32 [E, {hidden}]")
     num = router_weight.shape[0]
-    _need(router_bias is None or (router_bias.dtype == torch.float32 and router_bias.shape == (num,)
-                                  and router_bias.is_contiguous()), f"router_bias must be contiguous fp32 [{num}]")
-    _need(1 <= top_k <= num, f"top_k must be 1 to {num}, got {top_k}")
-    return _p(router_weight), int(router_weight.dtype == torch.float32), _p(router_bias), int(score == "sigmoid")
+    if router_bias is not None and (router_bias.dtype is not _FP32 or router_bias.shape != (num,) or not router_bias.is_contiguous()):
+        _refuse(f"router_bias must be contiguous fp32 [{num}]")
+    if not 1 <= top_k <= num:
+        _refuse(f"top_k must be 1 to {num}, got {top_k}")
+    return num, router_weight.data_ptr(), dtype is _FP32, _p(router_bias), score == "sigmoid"
 
 
 def moe_route(x: torch.Tensor, router_weight: torch.Tensor, top_k: int, *, score: str = "softmax",
@@ -721,20 +757,14 @@ def moe_route(x: torch.Tensor, router_weight: torch.Tensor, top_k: int, *, score
     the score alone, renormalised over the chosen ones if asked for, times
     ``routed_scale``.  Rows that ``token_mask`` (bool ``[T]``) leaves out get
     ids -1 and weights 0.  E <= 512, top_k <= 16, H a multiple of 32."""
-    _check_here(x, token_mask)
-    _need(x.dtype == torch.bfloat16, f"x must be bf16, got {x.dtype}")
-    _check_rows(x)
-    t, hidden = x.shape
-    wr, fp32, bias, sigmoid = _router_args(x, router_weight, router_bias, top_k, score)
-    _need(token_mask is None or (token_mask.dtype in (torch.bool, torch.uint8) and token_mask.shape == (t,)
-                                 and token_mask.is_contiguous()), f"token_mask must be contiguous bool [{t}]")
-    ids = torch.empty((t, top_k), dtype=torch.int32, device=x.device)
-    weights = torch.empty((t, top_k), dtype=torch.float32, device=x.device)
-    num = router_weight.shape[0]
+    dev, t, hidden, stride, at = _moe_rows(x, token_mask, router_weight, router_bias)
+    num, wr, fp32, bias, sigmoid = _router_args(hidden, router_weight, router_bias, top_k, score)
+    ids = torch.empty((t, top_k), dtype=_I32, device=x.device)
+    weights = torch.empty((t, top_k), dtype=_FP32, device=x.device)
     nbytes = lib().hca_moe_route_workspace_bytes(t, num)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    call("hca_moe_route", _p(ids), _p(weights), _p(x), x.stride(0), wr, fp32, bias, _p(token_mask), t, num, hidden, top_k,
-         sigmoid, int(renormalize), routed_scale, _p(ws), nbytes, _s())
+    ws = torch.empty(nbytes, dtype=_U8, device=x.device)
+    call("hca_moe_route", ids.data_ptr(), weights.data_ptr(), at, stride, wr, fp32, bias, _p(token_mask), t, num, hidden,
+         top_k, sigmoid, renormalize, routed_scale, ws.data_ptr(), nbytes, _stream(dev))
     return ids, weights
 
 
@@ -748,21 +778,20 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
     ``ids`` int32 ``[T, top_k]`` (ids outside ``[0, E)`` are skipped, as for the
     experts of another rank; an id may repeat), ``weights`` fp32 ``[T, top_k]``.
     Each chosen expert's weights are read once for all its tokens (of 64 at a
-    time).  Rows that ``token_mask`` leaves out come out as 0 and choose
-    nothing.  The gated product is rounded to bf16 once, its weight included;
-    sums are fp32."""
-    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, experts, shared, token_mask)
-    _check_here(ids, weights)
-    t, hidden = x.shape
-    _need(ids.dtype == torch.int32 and ids.dim() == 2 and ids.shape[0] == t and ids.is_contiguous()
-          and weights.dtype == torch.float32 and weights.shape == ids.shape and weights.is_contiguous(),
-          f"ids must be contiguous int32 [{t}, top_k] and weights fp32 alike")
+    time; again for each 16 tokens of one expert).  Rows that ``token_mask``
+    leaves out come out as 0 and choose nothing.  The gated product is rounded
+    to bf16 once, its weight included; sums are fp32."""
+    dev, t, hidden, stride, at = _moe_rows(x, token_mask, ids, weights)
+    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, dev, hidden, experts, shared)
+    if (ids.dtype is not _I32 or ids.dim() != 2 or ids.shape[0] != t or not ids.is_contiguous()
+            or weights.dtype is not _FP32 or weights.shape != ids.shape or not weights.is_contiguous()):
+        _refuse(f"ids must be contiguous int32 [{t}, top_k] and weights fp32 alike")
     top_k = ids.shape[1]
-    out = _rows_out(x, hidden, out)
+    out = _rows_out(x, dev, t, hidden, out)
     nbytes = lib().hca_moe_workspace_bytes(t, num, top_k, hidden, inner, shared_inner)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    call("hca_moe_experts", _p(out), out.stride(0), _p(x), x.stride(0), _p(ids), _p(weights), _p(token_mask), fmt, group,
-         *ptrs, t, num, hidden, inner, shared_inner, top_k, _p(ws), nbytes, _s())
+    ws = torch.empty(nbytes, dtype=_U8, device=x.device)
+    call("hca_moe_experts", out.data_ptr(), out.stride(0), at, stride, ids.data_ptr(), weights.data_ptr(), _p(token_mask), fmt,
+         group, *ptrs, t, num, hidden, inner, shared_inner, top_k, ws.data_ptr(), nbytes, _stream(dev))
     return out
 
 
@@ -771,18 +800,19 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts: MoEWeights
                shared: MoEWeights | None = None, token_mask: torch.Tensor | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
     """A whole mixture-of-experts layer for a few tokens (``moe_route`` then
-    ``moe_experts``) in one call; ``x`` and the result bf16 ``[T, H]``.  Its
-    scratch comes from the caching allocator on the current stream, so calls
-    on several streams do not meet."""
-    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, experts, shared, token_mask)
-    wr, fp32, bias, sigmoid = _router_args(x, router_weight, router_bias, top_k, score)
-    _need(router_weight.shape[0] == num, f"router_weight must have the {num} experts' rows")
-    t, hidden = x.shape
-    out = _rows_out(x, hidden, out)
+    ``moe_experts``) in one call of two launches; ``x`` and the result bf16
+    ``[T, H]``.  Its scratch comes from the caching allocator on the current
+    stream, so calls on several streams do not meet."""
+    dev, t, hidden, stride, at = _moe_rows(x, token_mask, router_weight, router_bias)
+    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, dev, hidden, experts, shared)
+    rows, wr, fp32, bias, sigmoid = _router_args(hidden, router_weight, router_bias, top_k, score)
+    if rows != num:
+        _refuse(f"router_weight must have the {num} experts' rows")
+    out = _rows_out(x, dev, t, hidden, out)
     nbytes = lib().hca_moe_workspace_bytes(t, num, top_k, hidden, inner, shared_inner)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    call("hca_moe_decode", _p(out), out.stride(0), _p(x), x.stride(0), wr, fp32, bias, sigmoid, int(renormalize),
-         routed_scale, _p(token_mask), fmt, group, *ptrs, t, num, hidden, inner, shared_inner, top_k, _p(ws), nbytes, _s())
+    ws = x.new_empty((nbytes + 1) // 2)
+    call("hca_moe_decode", out.data_ptr(), out.stride(0), at, stride, wr, fp32, bias, sigmoid, renormalize, routed_scale,
+         _p(token_mask), fmt, group, *ptrs, t, num, hidden, inner, shared_inner, top_k, ws.data_ptr(), nbytes, _stream(dev))
     return out
 
 
@@ -809,43 +839,58 @@ def apply_logit_penalties(logits: torch.Tensor, token_ids: torch.Tensor | None =
     and ``bias_values`` fp32 ``[R, M]`` (of an id listed twice the later
     counts); ids outside ``[0, V)``, like -1, are skipped.  ``allowed_bitmask``
     int32 ``[rows, ceil(V / 32)]``, bit ``v % 32`` of word ``v // 32``."""
-    _check_here(logits, token_ids, prompt_lens, seq_lens, repetition, frequency, presence, bias_ids, bias_values,
-                allowed_bitmask, req_index)
+    dev = _device_of(logits, token_ids, prompt_lens, seq_lens, repetition, frequency, presence, bias_ids, bias_values,
+                     allowed_bitmask, req_index)
     kind = _LOGIT_TYPES.get(logits.dtype, -1)
-    _need(kind >= 0, f"logits must be fp32, bf16 or fp16, got {logits.dtype}")
-    _need(logits.dim() == 2 and logits.shape[1] > 0 and (logits.shape[1] == 1 or logits.stride(1) == 1),
-          "logits must be [rows, V] with contiguous rows")
+    if kind < 0:
+        _refuse(f"logits must be fp32, bf16 or fp16, got {logits.dtype}")
+    if logits.dim() != 2:
+        _refuse("logits must be [rows, V]")
     rows, vocab = logits.shape
-    tables = [t for t in (token_ids, repetition, frequency, presence, bias_ids, bias_values) if t is not None]
-    reqs = tables[0].shape[0] if tables else rows
+    logits_stride, inner = logits.stride()
+    if vocab == 0 or (vocab > 1 and inner != 1):
+        _refuse("logits must be [rows, V] with contiguous rows")
+    reqs = rows
+    for t in (token_ids, repetition, frequency, presence, bias_ids):
+        if t is not None:
+            reqs = t.shape[0]
+            break
     for t in (repetition, frequency, presence):
-        _need(t is None or (t.dtype == torch.float32 and t.shape == (reqs,) and t.is_contiguous()),
-              f"penalties must be contiguous fp32 [{reqs}]")
+        if t is not None and (t.dtype is not _FP32 or t.shape != (reqs,) or not t.is_contiguous()):
+            _refuse(f"penalties must be contiguous fp32 [{reqs}]")
     if req_index is None:
-        _need(reqs == rows, f"{reqs} requests for {rows} rows need req_index")
-    else:
-        _need(req_index.dtype == torch.int32 and req_index.shape == (rows,) and req_index.is_contiguous(),
-              f"req_index must be contiguous int32 [{rows}]")
+        if reqs != rows:
+            _refuse(f"{reqs} requests for {rows} rows need req_index")
+    elif req_index.dtype is not _I32 or req_index.shape != (rows,) or not req_index.is_contiguous():
+        _refuse(f"req_index must be contiguous int32 [{rows}]")
     width = stride = 0
     if token_ids is not None:
-        _need(token_ids.dtype == torch.int32 and token_ids.dim() == 2 and token_ids.shape[0] == reqs
-              and (token_ids.shape[1] <= 1 or token_ids.stride(1) == 1), f"token_ids must be int32 [{reqs}, L] with contiguous rows")
+        if token_ids.dtype is not _I32 or token_ids.dim() != 2 or token_ids.shape[0] != reqs:
+            _refuse(f"token_ids must be int32 [{reqs}, L]")
+        width = token_ids.shape[1]
+        stride, inner = token_ids.stride()
+        if width > 1 and inner != 1:
+            _refuse("token_ids must have contiguous rows")
         for t in (prompt_lens, seq_lens):
-            _need(t is not None and t.dtype == torch.int32 and t.shape == (rows,) and t.is_contiguous(),
-                  f"prompt_lens and seq_lens must be contiguous int32 [{rows}]")
-        width, stride = token_ids.shape[1], token_ids.stride(0)
-    bias_width = bias_stride = 0
-    _need((bias_ids is None) == (bias_values is None), "bias_ids and bias_values come together")
+            if t is None or t.dtype is not _I32 or t.shape != (rows,) or not t.is_contiguous():
+                _refuse(f"prompt_lens and seq_lens must be contiguous int32 [{rows}]")
+    bias_width = 0
+    if (bias_ids is None) != (bias_values is None):
+        _refuse("bias_ids and bias_values come together")
     if bias_ids is not None:
-        _need(bias_ids.dtype == torch.int32 and bias_ids.dim() == 2 and bias_ids.shape[0] == reqs and bias_ids.is_contiguous()
-              and bias_values.dtype == torch.float32 and bias_values.shape == bias_ids.shape and bias_values.is_contiguous(),
-              f"bias_ids must be contiguous int32 [{reqs}, M] and bias_values fp32 alike")
-        bias_width = bias_stride = bias_ids.shape[1]
+        if (bias_ids.dtype is not _I32 or bias_ids.dim() != 2 or bias_ids.shape[0] != reqs or not bias_ids.is_contiguous()
+                or bias_values.dtype is not _FP32 or bias_values.shape != bias_ids.shape or not bias_values.is_contiguous()):
+            _refuse(f"bias_ids must be contiguous int32 [{reqs}, M] and bias_values fp32 alike")
+        bias_width = bias_ids.shape[1]
+    allowed_stride = 0
     if allowed_bitmask is not None:
-        _need(allowed_bitmask.dtype == torch.int32 and allowed_bitmask.shape == (rows, -(-vocab // 32))
-              and allowed_bitmask.stride(1) == 1, f"allowed_bitmask must be int32 [{rows}, {-(-vocab // 32)}] with contiguous rows")
-    call("hca_logit_penalties", _p(logits), logits.stride(0), kind, _p(req_index), reqs, _p(token_ids), stride, width,
+        words = (vocab + 31) // 32
+        if allowed_bitmask.dtype is not _I32 or allowed_bitmask.shape != (rows, words):
+            _refuse(f"allowed_bitmask must be int32 [{rows}, {words}]")
+        allowed_stride, inner = allowed_bitmask.stride()
+        if words > 1 and inner != 1:
+            _refuse("allowed_bitmask must have contiguous rows")
+    call("hca_logit_penalties", logits.data_ptr(), logits_stride, kind, _p(req_index), reqs, _p(token_ids), stride, width,
          _p(prompt_lens), _p(seq_lens), _p(repetition), _p(frequency), _p(presence), _p(bias_ids), _p(bias_values),
-         bias_stride, bias_width, _p(allowed_bitmask), allowed_bitmask.stride(0) if allowed_bitmask is not None else 0, rows,
-         vocab, _s())
+         bias_width, bias_width, _p(allowed_bitmask), allowed_stride, rows, vocab, _stream(dev))
     return logits
