@@ -10,8 +10,8 @@
 // texts crowd into spread over all of them.  Each CTA reads the row's whole
 // history (from L2 but for the first) and counts its own tokens in shared
 // memory; counts are whole numbers, so their order does not matter, and no
-// table lives in global memory.  Then a warp goes over a chunk at a time, a
-// lane a token, several chunks' loads under way.
+// table lives in global memory.  Then each warp lists the tokens seen among a
+// few hundred and its lanes share them out, so that their loads run together.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -21,9 +21,9 @@
 namespace hca {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kAhead = 8;  // chunks of a warp under way
-constexpr int kMostSlices = 1024;
+constexpr int kThreads = 1024;
+constexpr int kAhead = 4;  // logits of a lane under way
+constexpr int kSmem = 224 * 1024;
 
 __device__ __forceinline__ float load_logit(const float* p) { return *p; }
 __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -52,53 +52,64 @@ struct LogitArgs {
 };
 
 // A CTA's share of a row: chunks rank, rank + slices, ... of 32 tokens.  Tables
-// by local chunk: counts (16 bits where the history cannot hold more than
-// 65535 tokens, else 32), a word of prompt bits, a word of biased tokens' bits.
+// by local chunk: a word of prompt bits, a word of biased tokens' bits, counts
+// (16 bits where the history cannot hold more than 65535 tokens, else 32).
+template <typename Count>
+struct Tables {
+  static constexpr int kEntry = static_cast<int>(sizeof(Count));
+  static constexpr int kSpan = 16;  // tokens of a lane at a time
+  static constexpr int kListBytes = kThreads * kSpan * 2;
+  // chunks, rounded up so that every lane's span exists
+  static __host__ __device__ int64_t padded(int64_t chunks) { return (chunks + 15) / 16 * 16; }
+  static __host__ __device__ int64_t bytes(int64_t chunks) { return padded(chunks) * (8 + 32 * kEntry); }
+};
+
 template <typename T, typename Count>
-__global__ void __launch_bounds__(kThreads, 2) logit_penalty_kernel(LogitArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a) {
+  using Tab = Tables<Count>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int slices = 1 << a.slices_log2;
   const int64_t row = blockIdx.x >> a.slices_log2;
   const int rank = blockIdx.x & (slices - 1);
   const int all_chunks = (a.vocab + 31) / 32;
-  const int most = (all_chunks + slices - 1) / slices;  // the same for every CTA
-  const int chunks = (all_chunks - rank + slices - 1) / slices;
+  const int chunks = (all_chunks - rank + slices - 1) >> a.slices_log2;
+  const int padded = static_cast<int>(Tab::padded((all_chunks + slices - 1) >> a.slices_log2));
   uint32_t* prompt = reinterpret_cast<uint32_t*>(smem);
-  uint32_t* biased = prompt + most;
-  Count* count = reinterpret_cast<Count*>(smem + (8 * most + 15) / 16 * 16);
+  uint32_t* biased = prompt + padded;
+  Count* count = reinterpret_cast<Count*>(biased + padded);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  {
-    const int words = ((8 * most + 15) / 16 * 16 + 32 * most * static_cast<int>(sizeof(Count))) / 16;
-    for (int i = threadIdx.x; i < words; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-  }
+  uint16_t* list = reinterpret_cast<uint16_t*>(count + 32 * padded) + warp * 32 * Tab::kSpan;
+  for (int i = threadIdx.x; i < Tab::bytes(padded) / 16; i += kThreads)
+    reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   pdl_wait_and_release();
   const int64_t req = a.req_index == nullptr ? row : a.req_index[row];
   if (req < 0 || req >= a.num_reqs) return;  // the whole CTA
   T* logits = static_cast<T*>(a.logits) + row * a.stride;
   __syncthreads();
 
-  // v's local chunk and bit, if it is this CTA's
-  auto mine = [&](int32_t v, int& chunk, int& bit) -> bool {
-    const uint32_t c = static_cast<uint32_t>(v) >> 5;
-    chunk = static_cast<int>(c >> a.slices_log2), bit = v & 31;
-    return static_cast<uint32_t>(v) < static_cast<uint32_t>(a.vocab) && static_cast<int>(c & (slices - 1)) == rank;
+  // Whether v is this CTA's, and its place in the tables.
+  const uint32_t owner = static_cast<uint32_t>(rank) << 5, owner_mask = static_cast<uint32_t>(slices - 1) << 5;
+  const int shift = 5 + a.slices_log2;
+  auto mine = [&](int32_t v) {
+    return ((static_cast<uint32_t>(v) ^ owner) & owner_mask) == 0 && static_cast<uint32_t>(v) < static_cast<uint32_t>(a.vocab);
   };
+  auto place = [&](int32_t v) { return (v >> shift) * 32 + (v & 31); };
   if (a.token_ids != nullptr) {
     const int32_t* tokens = a.token_ids + req * a.token_stride;
-    const int seq_len = min(a.seq_lens[row], a.token_width), prompt_len = min(a.prompt_lens[row], seq_len);
+    const int seq_len = max(min(a.seq_lens[row], a.token_width), 0);
+    const int prompt_len = max(min(a.prompt_lens[row], seq_len), 0);
     auto see = [&](int32_t v, bool answer) {
-      int c, bit;
-      if (!mine(v, c, bit)) return;
-      if (!answer) atomicOr(prompt + c, 1u << bit);
-      else if constexpr (sizeof(Count) == 4) atomicAdd(reinterpret_cast<uint32_t*>(count) + 32 * c + bit, 1u);
+      if (!mine(v)) return;
+      const int at = place(v);
+      if (!answer) atomicOr(prompt + (at >> 5), 1u << (at & 31));
+      else if constexpr (Tab::kEntry == 4) atomicAdd(reinterpret_cast<uint32_t*>(count) + at, 1u);
       // two counts to a word: neither passes 65535, so none carries
-      else atomicAdd(reinterpret_cast<uint32_t*>(count) + 16 * c + (bit >> 1), bit & 1 ? 0x10000u : 1u);
+      else atomicAdd(reinterpret_cast<uint32_t*>(count) + (at >> 1), at & 1 ? 0x10000u : 1u);
     };
     // four tokens at a time from the first 16-byte boundary on
-    const int lead = static_cast<int>(-(reinterpret_cast<intptr_t>(tokens) >> 2) & 3);
-    const int head = min(lead, max(seq_len, 0));
+    const int head = min(static_cast<int>(-(reinterpret_cast<intptr_t>(tokens) >> 2) & 3), seq_len);
     if (static_cast<int>(threadIdx.x) < head) see(tokens[threadIdx.x], static_cast<int>(threadIdx.x) >= prompt_len);
-    const int quads = max(seq_len - head, 0) / 4;
+    const int quads = (seq_len - head) / 4, done = head + 4 * quads;
     const int4* body = reinterpret_cast<const int4*>(tokens + head);
 #pragma unroll 4
     for (int i = threadIdx.x; i < quads; i += kThreads) {
@@ -109,14 +120,13 @@ __global__ void __launch_bounds__(kThreads, 2) logit_penalty_kernel(LogitArgs a)
       see(v.z, at + 2 >= prompt_len);
       see(v.w, at + 3 >= prompt_len);
     }
-    const int done = head + 4 * quads;
     if (static_cast<int>(threadIdx.x) < seq_len - done)
       see(tokens[done + threadIdx.x], done + static_cast<int>(threadIdx.x) >= prompt_len);
   }
   const int32_t* bias_ids = a.bias_ids + req * a.bias_stride;
   for (int i = threadIdx.x; i < a.bias_width; i += kThreads) {
-    int c, bit;
-    if (mine(bias_ids[i], c, bit)) atomicOr(biased + c, 1u << bit);
+    const int v = bias_ids[i];
+    if (mine(v)) atomicOr(biased + (place(v) >> 5), 1u << (v & 31));
   }
   __syncthreads();
 
@@ -129,67 +139,94 @@ __global__ void __launch_bounds__(kThreads, 2) logit_penalty_kernel(LogitArgs a)
     if (n != 0) x = x - freq * static_cast<float>(n) - pres;
     return x;
   };
-  for (int c0 = warp; c0 < chunks; c0 += kAhead * (kThreads / 32)) {
-    // what is to be done with the lane's token of each chunk: 0 nothing, 1 penalties, 2 -inf
-    int what[kAhead];
-    uint32_t n[kAhead];
-    bool seen[kAhead];
-    float x[kAhead];
-    uint32_t word[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int c = c0 + j * (kThreads / 32);
-      word[j] = ~0u;
-      if (allowed != nullptr && c < chunks) word[j] = static_cast<uint32_t>(allowed[c * slices + rank]);
+  // the token of a place, and back to its logit
+  auto token = [&](int at) { return ((at >> 5 << a.slices_log2) + rank) * 32 + (at & 31); };
+
+  // Masked places, a warp to 32 chunks: a lane loads a chunk's word, then is a bit of each.
+  if (allowed != nullptr) {
+    for (int c0 = warp * 32; c0 < chunks; c0 += kThreads) {
+      const uint32_t words = c0 + lane < chunks ? static_cast<uint32_t>(allowed[((c0 + lane) << a.slices_log2) + rank]) : ~0u;
+      T* at = logits + token(c0 * 32) + lane;
+      const int step = 32 << a.slices_log2;
+#pragma unroll 8
+      for (int j = 0; j < 32; ++j, at += step) {
+        const uint32_t word = __shfl_sync(0xffffffffu, words, j);
+        if (!(word >> lane & 1) && token((c0 + j) * 32) + lane < a.vocab) store_logit(at, -INFINITY);
+      }
     }
+  }
+  // Seen, allowed and not biased ones: a lane finds those of kSpan places, the
+  // warp lists them and shares them out.
+  for (int c0 = warp * Tab::kSpan; c0 < chunks; c0 += kThreads / 32 * Tab::kSpan) {
+    const int base = c0 * 32 + lane * Tab::kSpan, c = base >> 5, bit = base & 31;
+    uint32_t bits = prompt[c] >> bit;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int c = c0 + j * (kThreads / 32);
-      what[j] = 0, n[j] = 0, x[j] = 0.0f, seen[j] = false;
-      const int v = (c * slices + rank) * 32 + lane;
-      if (c >= chunks || v >= a.vocab) continue;
-      n[j] = count[32 * c + lane];
-      seen[j] = n[j] != 0 || (prompt[c] >> lane & 1);
-      if (!(word[j] >> lane & 1)) what[j] = 2;
-      else if (seen[j] && !(biased[c] >> lane & 1)) what[j] = 1;
-      if (what[j] == 1) x[j] = load_logit(logits + v);
-    }
+    for (int i = 0; i < Tab::kSpan * Tab::kEntry / 16; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(count + base)[i];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int v = ((c0 + j * (kThreads / 32)) * slices + rank) * 32 + lane;
-      if (what[j] != 0) store_logit(logits + v, what[j] == 2 ? -INFINITY : penalise(x[j], n[j], seen[j]));
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (Tab::kEntry == 4) bits |= w[j] != 0 ? 1u << (4 * i + j) : 0u;
+        else bits |= ((w[j] & 0xffffu) != 0 ? 1u << (8 * i + 2 * j) : 0u) | (w[j] > 0xffffu ? 2u << (8 * i + 2 * j) : 0u);
+      }
     }
+    bits &= ~(biased[c] >> bit) & ((1u << Tab::kSpan) - 1);
+    if (allowed != nullptr && bits != 0) bits &= static_cast<uint32_t>(allowed[(c << a.slices_log2) + rank]) >> bit;
+    const int mine_n = __popc(bits);
+    int before = mine_n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, before, 31);
+    before -= mine_n;
+    for (; bits != 0; bits &= bits - 1) list[before++] = static_cast<uint16_t>(base - c0 * 32 + __ffs(bits) - 1);
+    __syncwarp();
+    for (int i0 = 0; i0 < total; i0 += 32 * kAhead) {
+      float x[kAhead];
+      int at[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + 32 * j + lane;
+        at[j] = i < total ? c0 * 32 + list[i] : -1;
+        if (at[j] >= 0) x[j] = load_logit(logits + token(at[j]));
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (at[j] >= 0) store_logit(logits + token(at[j]), penalise(x[j], count[at[j]], true));
+    }
+    __syncwarp();
   }
   for (int i = threadIdx.x; i < a.bias_width; i += kThreads) {
     const int v = bias_ids[i];
-    int c, bit;
-    if (!mine(v, c, bit)) continue;
+    if (!mine(v)) continue;
     bool last = true;  // an id listed twice: the later entry counts
     for (int j = i + 1; j < a.bias_width; ++j) last = last && bias_ids[j] != v;
-    if (!last || (allowed != nullptr && !(static_cast<uint32_t>(allowed[v >> 5]) >> bit & 1))) continue;
-    const uint32_t k = count[32 * c + bit];
+    if (!last || (allowed != nullptr && !(static_cast<uint32_t>(allowed[v >> 5]) >> (v & 31) & 1))) continue;
+    const int at = place(v);
+    const uint32_t n = count[at];
     const float x = load_logit(logits + v) + a.bias_values[req * a.bias_stride + i];
-    store_logit(logits + v, penalise(x, k, k != 0 || (prompt[c] >> bit & 1)));
+    store_logit(logits + v, penalise(x, n, n != 0 || (prompt[at >> 5] >> (at & 31) & 1)));
   }
 }
 
 template <typename T, typename Count>
 int launch(LogitArgs a, int rows, cudaStream_t s) {
-  const int chunks = (a.vocab + 31) / 32, sms = device_sm_count();
-  auto bytes = [&](int log2) {
-    const int64_t most = (chunks + (1 << log2) - 1) >> log2;
-    return (8 * most + 15) / 16 * 16 + 32 * most * static_cast<int64_t>(sizeof(Count));
-  };
-  // Slices of a row: so many that two CTAs fit an SM, and while SMs would be
-  // left without one, more, down to 64 chunks each.
+  using Tab = Tables<Count>;
+  const int64_t chunks = (static_cast<int64_t>(a.vocab) + 31) / 32, sms = device_sm_count();
+  auto bytes = [&](int log2) { return Tab::bytes((chunks + (1 << log2) - 1) >> log2) + Tab::kListBytes; };
+  // Slices of a row: as few as shared memory allows, since each reads the
+  // history; while they leave half the SMs without work twice as many, down to
+  // 64 chunks each.
   a.slices_log2 = 0;
-  while (bytes(a.slices_log2) > 108 * 1024 ||
-         ((static_cast<int64_t>(rows) << a.slices_log2) < 2 * sms && (chunks >> a.slices_log2) >= 128))
+  while (bytes(a.slices_log2) > kSmem ||
+         ((static_cast<int64_t>(rows) << (a.slices_log2 + 1)) <= sms && (chunks >> a.slices_log2) >= 128))
     ++a.slices_log2;
-  if (1 << a.slices_log2 > kMostSlices) return HCA_E_UNSUPPORTED;
+  if ((static_cast<int64_t>(rows) << a.slices_log2) > INT32_MAX) return HCA_E_INVALID;
   static bool done[kMaxDevices] = {};
-  if (set_func_attr_once(logit_penalty_kernel<T, Count>, cudaFuncAttributeMaxDynamicSharedMemorySize, 108 * 1024,
-                         done) != HCA_OK)
+  if (set_func_attr_once(logit_penalty_kernel<T, Count>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done) !=
+      HCA_OK)
     return HCA_E_CUDA;
   return launch_pdl(logit_penalty_kernel<T, Count>, dim3(static_cast<unsigned>(rows) << a.slices_log2), dim3(kThreads),
                     static_cast<size_t>(bytes(a.slices_log2)), s, a);
@@ -218,7 +255,6 @@ extern "C" int hca_logit_penalties(void* logits, int64_t logits_stride, int32_t 
   HCA_CHECK_ARG(req_index || num_reqs >= num_rows);
   HCA_CHECK_ARG(token_ids == nullptr || (prompt_lens && seq_lens));
   HCA_CHECK_ARG(bias_width == 0 || (bias_ids && bias_values));
-  HCA_CHECK_ARG(num_rows <= INT32_MAX / kMostSlices);
   LogitArgs a;
   a.logits = logits, a.stride = logits_stride, a.req_index = req_index, a.num_reqs = num_reqs;
   a.token_ids = token_ids, a.token_stride = token_stride, a.token_width = token_width;
