@@ -22,7 +22,7 @@ namespace hca {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kAhead = 4;  // logits of a lane under way
+constexpr int kAhead = 2;  // logits of a lane under way
 constexpr int kSmem = 224 * 1024;
 
 __device__ __forceinline__ float load_logit(const float* p) { return *p; }
@@ -68,6 +68,7 @@ template <typename T, typename Count>
 __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a) {
   using Tab = Tables<Count>;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int next_span;
   const int slices = 1 << a.slices_log2;
   const int64_t row = blockIdx.x >> a.slices_log2;
   const int rank = blockIdx.x & (slices - 1);
@@ -81,6 +82,7 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
   uint16_t* list = reinterpret_cast<uint16_t*>(count + 32 * padded) + warp * 32 * Tab::kSpan;
   for (int i = threadIdx.x; i < Tab::bytes(padded) / 16; i += kThreads)
     reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0) next_span = 0;
   pdl_wait_and_release();
   const int64_t req = a.req_index == nullptr ? row : a.req_index[row];
   if (req < 0 || req >= a.num_reqs) return;  // the whole CTA
@@ -130,12 +132,12 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
   }
   __syncthreads();
 
-  const float rep = a.repetition == nullptr ? 1.0f : a.repetition[req];
+  const float rep = a.repetition == nullptr ? 1.0f : a.repetition[req], inverse = 1.0f / rep;
   const float freq = a.frequency == nullptr ? 0.0f : a.frequency[req];
   const float pres = a.presence == nullptr ? 0.0f : a.presence[req];
   const int32_t* allowed = a.allowed == nullptr ? nullptr : a.allowed + row * a.allowed_stride;
   auto penalise = [&](float x, uint32_t n, bool seen) {
-    if (seen) x = x > 0.0f ? x / rep : x * rep;
+    if (seen) x = x * (x > 0.0f ? inverse : rep);
     if (n != 0) x = x - freq * static_cast<float>(n) - pres;
     return x;
   };
@@ -143,35 +145,44 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
   auto token = [&](int at) { return ((at >> 5 << a.slices_log2) + rank) * 32 + (at & 31); };
 
   // Masked places, a warp to 32 chunks: a lane loads a chunk's word, then is a bit of each.
-  if (allowed != nullptr) {
+  auto close = [&]() {
     for (int c0 = warp * 32; c0 < chunks; c0 += kThreads) {
-      const uint32_t words = c0 + lane < chunks ? static_cast<uint32_t>(allowed[((c0 + lane) << a.slices_log2) + rank]) : ~0u;
+      const int own = c0 + lane;
+      uint32_t words = own < chunks ? static_cast<uint32_t>(allowed[(own << a.slices_log2) + rank]) : ~0u;
+      const int over = token(own * 32) + 32 - a.vocab;  // places past the vocabulary's end
+      if (over > 0 && over < 32) words |= ~0u << (32 - over);
       T* at = logits + token(c0 * 32) + lane;
-      const int step = 32 << a.slices_log2;
-#pragma unroll 8
-      for (int j = 0; j < 32; ++j, at += step) {
-        const uint32_t word = __shfl_sync(0xffffffffu, words, j);
-        if (!(word >> lane & 1) && token((c0 + j) * 32) + lane < a.vocab) store_logit(at, -INFINITY);
-      }
+      const uint32_t bit = 1u << lane;
+      const int step = 1 << shift;
+#pragma unroll 16
+      for (int j = 0; j < 32; ++j, at += step)
+        if (!(__shfl_sync(0xffffffffu, words, j) & bit)) store_logit(at, -INFINITY);
     }
-  }
+  };
   // Seen, allowed and not biased ones: a lane finds those of kSpan places, the
   // warp lists them and shares them out.
-  for (int c0 = warp * Tab::kSpan; c0 < chunks; c0 += kThreads / 32 * Tab::kSpan) {
+  if (allowed != nullptr && (warp & 1)) close();  // half the warps first, half last: stores beside latency
+  // whoever is free takes the next span: the low ids' are the longest
+  for (;;) {
+    int c0 = lane == 0 ? atomicAdd(&next_span, Tab::kSpan) : 0;
+    c0 = __shfl_sync(0xffffffffu, c0, 0);
+    if (c0 >= chunks) break;
     const int base = c0 * 32 + lane * Tab::kSpan, c = base >> 5, bit = base & 31;
-    uint32_t bits = prompt[c] >> bit;
+    uint32_t may = ~0u;
+    if (allowed != nullptr && c < chunks) may = static_cast<uint32_t>(allowed[(c << a.slices_log2) + rank]);
+    uint32_t bits = prompt[c] >> bit, pairs = 0;
 #pragma unroll
     for (int i = 0; i < Tab::kSpan * Tab::kEntry / 16; ++i) {
       const uint4 v = reinterpret_cast<const uint4*>(count + base)[i];
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (Tab::kEntry == 4) bits |= w[j] != 0 ? 1u << (4 * i + j) : 0u;
-        else bits |= ((w[j] & 0xffffu) != 0 ? 1u << (8 * i + 2 * j) : 0u) | (w[j] > 0xffffu ? 2u << (8 * i + 2 * j) : 0u);
+        if constexpr (Tab::kEntry == 4) bits |= min(w[j], 1u) << (4 * i + j);
+        else pairs |= __vminu2(w[j], 0x00010001u) << (8 * i + 2 * j);  // even places from bit 0 on, odd ones from bit 16
       }
     }
-    bits &= ~(biased[c] >> bit) & ((1u << Tab::kSpan) - 1);
-    if (allowed != nullptr && bits != 0) bits &= static_cast<uint32_t>(allowed[(c << a.slices_log2) + rank]) >> bit;
+    bits |= (pairs & 0x5555u) | (pairs >> 15 & 0xaaaau);
+    bits &= (may & ~biased[c]) >> bit & ((1u << Tab::kSpan) - 1);
     const int mine_n = __popc(bits);
     int before = mine_n;
 #pragma unroll
@@ -184,8 +195,8 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
     for (; bits != 0; bits &= bits - 1) list[before++] = static_cast<uint16_t>(base - c0 * 32 + __ffs(bits) - 1);
     __syncwarp();
     for (int i0 = 0; i0 < total; i0 += 32 * kAhead) {
-      float x[kAhead];
       int at[kAhead];
+      float x[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int i = i0 + 32 * j + lane;
@@ -198,16 +209,18 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
     }
     __syncwarp();
   }
+  if (allowed != nullptr && !(warp & 1)) close();
   for (int i = threadIdx.x; i < a.bias_width; i += kThreads) {
     const int v = bias_ids[i];
     if (!mine(v)) continue;
     bool last = true;  // an id listed twice: the later entry counts
-    for (int j = i + 1; j < a.bias_width; ++j) last = last && bias_ids[j] != v;
+#pragma unroll 8
+    for (int j = i + 1; j < a.bias_width; ++j) last &= bias_ids[j] != v;
     if (!last || (allowed != nullptr && !(static_cast<uint32_t>(allowed[v >> 5]) >> (v & 31) & 1))) continue;
     const int at = place(v);
     const uint32_t n = count[at];
-    const float x = load_logit(logits + v) + a.bias_values[req * a.bias_stride + i];
-    store_logit(logits + v, penalise(x, n, n != 0 || (prompt[at >> 5] >> (at & 31) & 1)));
+    const float y = load_logit(logits + v) + a.bias_values[req * a.bias_stride + i];
+    store_logit(logits + v, penalise(y, n, n != 0 || (prompt[at >> 5] >> (at & 31) & 1)));
   }
 }
 
