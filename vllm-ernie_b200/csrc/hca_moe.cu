@@ -178,7 +178,7 @@ struct Scratch {
 
 int check_matrix(const MoeMatrix& m, int format) {
   HCA_CHECK_ARG(m.data && aligned(m.data, 16));
-  HCA_CHECK_ARG(format == HCA_WEIGHT_BF16 || (m.scale && aligned(m.scale, format == HCA_WEIGHT_FP8 ? 4 : 2)));
+  HCA_CHECK_ARG(format == HCA_WEIGHT_BF16 || (m.scale && aligned(m.scale, 4) && aligned(m.zero, 4)));
   return HCA_OK;
 }
 

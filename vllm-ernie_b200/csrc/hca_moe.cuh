@@ -14,6 +14,7 @@ constexpr int kMoeTokens = 64;    // tokens of one pass; more run as further pas
 constexpr int kMoeTopK = 16;      // most experts a token may choose
 constexpr int kMoeExperts = 512;  // most experts of a layer
 constexpr int kMoePairs = kMoeTokens * (kMoeTopK + 1);  // with the shared expert's
+
 // hca_device_error bit of the layer's grid barrier
 constexpr int kErrMoe = 1 << 6;
 

@@ -146,22 +146,6 @@ __device__ __forceinline__ bool grid_wait(uint32_t* barrier, uint32_t phase, int
   return __syncthreads_and(ok || threadIdx.x != 0);
 }
 
-// Row `row` of matrix e of a stack of matrices with n rows of k.
-template <int F>
-__device__ __forceinline__ void set_row(WCursor<F>& cur, int r, const MoeMatrix& m, int64_t e, int n, int row, int k) {
-  using W = WTraits<F>;
-  const int64_t at = e * n + row;
-  cur.data[r] = m.data + at * W::row_bytes(k) + (threadIdx.x & 3) * 4 * W::kWords;
-  if constexpr (W::kIs4) {
-    const int groups = k / W::kGroupK;
-    cur.scale[r] = static_cast<const __nv_bfloat16*>(m.scale) + at * groups;
-    cur.zero[r] = m.zero == nullptr ? nullptr : m.zero + at * groups;
-  } else if constexpr (F == kWFp8) {
-    const int64_t kb = (k + 127) / 128, nb = (n + 127) / 128;
-    cur.scale[r] = static_cast<const float*>(m.scale) + (e * nb + row / 128) * kb;
-  }
-}
-
 struct Shape {
   int up_warps, down_warps;  // warps that share a tile of either product
   int dense;                 // the first product's columns are the tokens, the same for every expert
@@ -178,15 +162,20 @@ struct Product {
   const MoePass& p;
   const MoeWeights& w;
   const P& pl;
-  uint8_t* smem;
+  uint8_t *smem, *scale_smem;
   TileGroup g;
   bool dense;
   int per_cta, tiles, pairs, from, to, end;  // [from, to) is the segment
-  int first_entry, first_tile;               // of the group in the segment
-  TileRing<F> ring;
+  int first_entry;
+  // a tile of the segment: this group's first, next to load, next to fetch
+  // scales of, and now consumed
+  struct Place {
+    int entry, tile;
+  } first, loading, fetching, now;
 
-  __device__ __forceinline__ Product(const MoePass& p_, const MoeWeights& w_, const P& pl_, uint8_t* smem_, int warps, bool dense_)
-      : p(p_), w(w_), pl(pl_), smem(smem_), g(warps), dense(dense_) {
+  __device__ __forceinline__ Product(const MoePass& p_, const MoeWeights& w_, const P& pl_, uint8_t* smem_,
+                                     uint8_t* scale_smem_, int warps, bool dense_)
+      : p(p_), w(w_), pl(pl_), smem(smem_), scale_smem(scale_smem_), g(warps), dense(dense_) {
     per_cta = kWarps / g.warps;
     tiles = kUp ? p.inner / 8 : p.hidden / 16;  // of a routed entry
     pairs = p.tokens * p.routing.top_k;
@@ -199,25 +188,54 @@ struct Product {
   __device__ __forceinline__ int k_of(int entry) const {
     return kUp ? p.hidden : entry >= pl.routed ? p.shared_inner : p.inner;
   }
-  // The item `by` after (entry, tile).
-  __device__ __forceinline__ void move(int& entry, int& tile, int by) const {
-    tile += by;
-    for (int n = tiles_of(entry); tile >= n && entry + 1 < pl.entries; n = tiles_of(entry)) tile -= n, ++entry;
+  __device__ __forceinline__ void move(Place& at, int by) const {
+    at.tile += by;
+    for (int n = tiles_of(at.entry); at.tile >= n && at.entry + 1 < pl.entries; n = tiles_of(at.entry)) at.tile -= n, ++at.entry;
   }
-  __device__ __forceinline__ void rows(WCursor<F>& cur, int entry, int tile) const {
-    const bool shared = entry >= pl.routed;
-    const int e = shared ? 0 : pl.expert[entry], row = (threadIdx.x & 31) >> 2;
-    if (kUp) {
-      const int inner = shared ? p.shared_inner : p.inner;
-      const MoeMatrix& m = shared ? w.shared13 : w.w13;
-      set_row<F>(cur, 0, m, e, 2 * inner, tile * 8 + row, p.hidden);
-      set_row<F>(cur, 1, m, e, 2 * inner, inner + tile * 8 + row, p.hidden);
-    } else {
-      const MoeMatrix& m = shared ? w.shared2 : w.w2;
-      set_row<F>(cur, 0, m, e, p.hidden, tile * 16 + row, k_of(entry));
-      set_row<F>(cur, 1, m, e, p.hidden, tile * 16 + 8 + row, k_of(entry));
+  // The matrix of a tile's rows, and the number of its fragment row r.
+  __device__ __forceinline__ const MoeMatrix& matrix(const Place& at, int64_t& e) const {
+    const bool shared = at.entry >= pl.routed;
+    e = shared ? 0 : pl.expert[at.entry];
+    return kUp ? (shared ? w.shared13 : w.w13) : (shared ? w.shared2 : w.w2);
+  }
+  __device__ __forceinline__ int rows_of(int entry) const {
+    return kUp ? 2 * (entry >= pl.routed ? p.shared_inner : p.inner) : p.hidden;
+  }
+  __device__ __forceinline__ int row(const Place& at, int r) const {
+    if (!kUp) return at.tile * 16 + r;
+    return at.tile * 8 + (r < 8 ? r : r - 8 + rows_of(at.entry) / 2);
+  }
+  // What the ring asks of its source.
+  __device__ __forceinline__ void rows(WCursor<F>& cur, int i) {
+    if (i > 0) move(loading, per_cta);
+    int64_t e;
+    const MoeMatrix& m = matrix(loading, e);
+    const int n = rows_of(loading.entry), k = k_of(loading.entry), lane = threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int at = row(loading, (lane >> 2) + 8 * r);
+      cur.data[r] = m.data + (e * n + at) * W::row_bytes(k) + (lane & 3) * 16;
+      if constexpr (F == kWFp8)
+        cur.scale[r] = static_cast<const float*>(m.scale) + (e * ((n + 127) / 128) + at / 128) * ((k + 127) / 128);
     }
   }
+  __device__ __forceinline__ bool zeros() const { return (kUp ? w.w13.zero : w.w2.zero) != nullptr || (kUp ? w.shared13.zero : w.shared2.zero) != nullptr; }
+  __device__ __forceinline__ WScales scales_of(const Place& at, int r) const {
+    int64_t e;
+    const MoeMatrix& m = matrix(at, e);
+    const int n = rows_of(at.entry), k = k_of(at.entry);
+    const uint8_t* s = static_cast<const uint8_t*>(m.scale);
+    const int groups = k / W::kGroupK;
+    const int64_t first_group = (e * n + row(at, r)) * groups;
+    const int64_t all = static_cast<int64_t>(at.entry >= pl.routed ? 1 : p.routing.experts) * n * groups;
+    return {s + 2 * first_group, s + 2 * all, m.zero == nullptr ? nullptr : m.zero + first_group, m.zero + all};
+  }
+  __device__ __forceinline__ WScales scales(int i, int r) {
+    if (i > 0) move(fetching, per_cta);
+    return scales_of(fetching, r);
+  }
+  __device__ __forceinline__ WScales here(int, int r) const { return scales_of(now, r); }
+
   __device__ __forceinline__ __nv_bfloat16* h_row(int pair) const {
     return pair < pairs ? p.h + static_cast<int64_t>(pair) * p.inner
                         : p.h + static_cast<int64_t>(pairs) * p.inner + static_cast<int64_t>(pair - pairs) * p.shared_inner;
@@ -226,34 +244,30 @@ struct Product {
 
   // Starts the loads of the next segment, the run of tiles that one layout of
   // columns serves: all with dense columns, else those of one entry.
-  __device__ __forceinline__ bool start() {
+  template <typename Ring>
+  __device__ __forceinline__ bool start(Ring& ring) {
     from = to;
     if (from >= end) return false;
     const int routed_items = pl.routed * tiles;
-    if (from < routed_items) first_entry = from / tiles, first_tile = from - first_entry * tiles;
+    int tile;
+    if (from < routed_items) first_entry = from / tiles, tile = from - first_entry * tiles;
     else {
       const int n = tiles_of(pl.routed);
-      first_entry = (from - routed_items) / n, first_tile = from - routed_items - first_entry * n;
+      first_entry = (from - routed_items) / n, tile = from - routed_items - first_entry * n;
       first_entry += pl.routed;
     }
-    to = dense ? end : min(end, from - first_tile + tiles_of(first_entry));
-    int e = first_entry, t = first_tile, at = 0;
-    move(e, t, g.id);
-    const int count = to - from > g.id ? (to - from - g.id + per_cta - 1) / per_cta : 0;
-    load_entry = e, load_tile = t;
-    (void)at;
-    ring.start(k_of(first_entry), g, count, [this](WCursor<F>& cur, int i) { next_rows(cur, i); });
+    to = dense ? end : min(end, from - tile + tiles_of(first_entry));
+    first = {first_entry, tile};
+    move(first, g.id);
+    loading = fetching = now = first;
+    ring.start(k_of(first_entry), g, to - from > g.id ? (to - from - g.id + per_cta - 1) / per_cta : 0, scale_smem, *this);
     return true;
-  }
-  int load_entry, load_tile;
-  __device__ __forceinline__ void next_rows(WCursor<F>& cur, int i) {
-    if (i > 0) move(load_entry, load_tile, per_cta);
-    rows(cur, load_entry, load_tile);
   }
 
   // Lays out the segment's columns and consumes its tiles.  Both ends are
   // block barriers for the columns.
-  __device__ __forceinline__ void run(TileSums<NB>& ts) {
+  template <typename Ring>
+  __device__ __forceinline__ void run(Ring& ring, TileSums<NB>& ts) {
     const int k = k_of(first_entry), l0 = pl.start[first_entry];
     const int columns = dense ? p.tokens : pl.start[first_entry + 1] - l0;
     const int live = (columns + kWidth - 1) / kWidth;
@@ -264,52 +278,52 @@ struct Product {
       const int pair = pl.pair[l0 + col];
       return kUp ? p.x + token(pair) * p.x_stride : h_row(pair);
     });
-    int entry = first_entry, tile = first_tile;
-    move(entry, tile, g.id);
     float acc[NB][4] = {};
     auto finish = [&](int, const float* sums) {
       constexpr int kCols = kUp ? 8 : 16;
-      const int s0 = pl.start[entry], n = (pl.start[entry + 1] - s0) * kCols;
+      const int s0 = pl.start[now.entry], n = (pl.start[now.entry + 1] - s0) * kCols;
       for (int i = g.thread(); i < n; i += g.threads()) {
         const int pair = pl.pair[s0 + i / kCols], c = i % kCols;
         const int col = dense ? token(pair) : i / kCols;
         const float v = TileSums<NB>::sum(sums, g, c, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
         if (kUp) {
           const float up = TileSums<NB>::sum(sums, g, c + 8, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
-          h_row(pair)[tile * 8 + c] = __float2bfloat16_rn(v / (1.0f + expf(-v)) * up * pl.weight[pair]);
+          h_row(pair)[now.tile * 8 + c] = __float2bfloat16_rn(v / (1.0f + expf(-v)) * up * pl.weight[pair]);
         } else {
-          p.part[static_cast<int64_t>(pair) * p.hidden + tile * 16 + c] = v;
+          p.part[static_cast<int64_t>(pair) * p.hidden + now.tile * 16 + c] = v;
         }
       }
-      move(entry, tile, per_cta);
+      move(now, per_cta);
     };
-    auto next = [this](WCursor<F>& cur, int i) { next_rows(cur, i); };
-    if (NB > 1 && live == 1) ring.template run<1>(xt, g, ts, acc, next, finish);
-    else ring.template run<NB>(xt, g, ts, acc, next, finish);
+    if (NB > 1 && live == 1) ring.template run<1>(xt, g, ts, acc, *this, finish);
+    else ring.template run<NB>(xt, g, ts, acc, *this, finish);
     __syncthreads();
   }
 };
 
 template <int F, int NB, int kWidth>
-__global__ void __launch_bounds__(kThreads, 1) moe_layer_kernel(MoePass p, MoeWeights w, Shape shape) {
+__global__ void __launch_bounds__(kThreads, 1)
+    moe_layer_kernel(MoePass p, MoeWeights w, Shape shape) {
   using X = XTile<F, __nv_bfloat16, NB, kWidth>;
   __shared__ Plan<NB * kWidth> pl;
   extern __shared__ __align__(16) uint8_t smem[];
   build_plan(pl, p);
-  const int k_max = max(p.hidden, max(p.inner, p.shared_inner));
-  TileSums<NB> ts(smem + X::bytes(WTraits<F>::units(k_max)));
+  TileRing<F, __nv_bfloat16> ring;
+  uint8_t* sums = smem + X::bytes(WTraits<F>::units(max(p.hidden, max(p.inner, p.shared_inner))));
+  TileSums<NB> ts(sums);
+  uint8_t* scales = sums + TileSums<NB>::bytes(kWarps);
   {
-    Product<F, NB, kWidth, true> up(p, w, pl, smem, shape.up_warps, shape.dense);
-    while (up.start()) up.run(ts);
+    Product<F, NB, kWidth, true> up(p, w, pl, smem, scales, shape.up_warps, shape.dense);
+    while (up.start(ring)) up.run(ring, ts);
   }
   grid_arrive(p.barrier);
   {
-    Product<F, NB, kWidth, false> down(p, w, pl, smem, shape.down_warps, false);
-    bool more = down.start();
+    Product<F, NB, kWidth, false> down(p, w, pl, smem, scales, shape.down_warps, false);
+    bool more = down.start(ring);
     if (!grid_wait(p.barrier, 1, p.error)) return;
     while (more) {
-      down.run(ts);
-      more = down.start();
+      down.run(ring, ts);
+      more = down.start(ring);
     }
   }
   grid_arrive(p.barrier);
@@ -333,44 +347,51 @@ __global__ void __launch_bounds__(kThreads, 1) moe_layer_kernel(MoePass p, MoeWe
   }
 }
 
+// Launches with entries of NB blocks of kWidth columns if shared memory holds them.
 template <int F, int NB, int kWidth>
-constexpr int64_t smem_bytes(int units) {
-  return XTile<F, __nv_bfloat16, NB, kWidth>::bytes(units) + TileSums<NB>::bytes(kWarps);
-}
-
-template <int F, int NB, int kWidth>
-int launch(const MoePass& p, const MoeWeights& w, int units, cudaStream_t s) {
+bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   using W = WTraits<F>;
   const int sms = device_sm_count();
+  const int inner = std::max(p.inner, p.shared_inner);
+  const int64_t columns = XTile<F, __nv_bfloat16, NB, kWidth>::bytes(W::units(std::max(p.hidden, inner))) +
+                          TileSums<NB>::bytes(kWarps);
+  const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr || w.shared13.zero != nullptr || w.shared2.zero != nullptr;
+  auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
   // Warps to a tile: as few as leave every group of every SM two tiles (if
-  // every pair chose another expert), but at least one unit a warp.
-  auto warps = [&](int64_t tiles, int64_t shared_tiles, int least_units) {
+  // every pair chose another expert) and room for the scales, but at least four
+  // units a warp (one step of its ring), or one where the tiles are too few to
+  // fill the machine otherwise.
+  auto warps = [&](int64_t tiles, int64_t shared_tiles, int k, int least_k) {
     const int64_t n = std::min(p.routing.experts, p.tokens * p.routing.top_k) * tiles + shared_tiles;
     int gw = 1;
-    while (gw < kWarps && n < 2ll * sms * (kWarps / gw) && 2 * gw <= least_units) gw *= 2;
+    while (gw < kWarps && 2 * gw <= W::units(least_k) &&
+           (n < (W::units(least_k) >= 8 * gw ? 2ll : 1ll) * sms * (kWarps / gw) || columns + scales(k, gw) > kSmem))
+      gw *= 2;
     return gw;
   };
   Shape shape;
-  shape.up_warps = warps(p.inner / 8, p.shared_inner / 8, W::units(p.hidden));
-  shape.down_warps = warps(p.hidden / 16, p.shared_inner > 0 ? p.hidden / 16 : 0,
-                           W::units(p.shared_inner > 0 ? std::min(p.inner, p.shared_inner) : p.inner));
+  shape.up_warps = warps(p.inner / 8, p.shared_inner / 8, p.hidden, p.hidden);
+  shape.down_warps = warps(p.hidden / 16, p.shared_inner > 0 ? p.hidden / 16 : 0, inner,
+                           p.shared_inner > 0 ? std::min(p.inner, p.shared_inner) : p.inner);
   // columns that hold every token serve every expert as they are
   shape.dense = p.tokens <= NB * kWidth;
+  const int64_t smem = columns + std::max(scales(p.hidden, shape.up_warps), scales(inner, shape.down_warps));
+  if (smem > kSmem) return false;
   static bool done[kMaxDevices] = {};
-  if (set_func_attr_once(moe_layer_kernel<F, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done) !=
-      HCA_OK)
-    return HCA_E_CUDA;
+  rc = set_func_attr_once(moe_layer_kernel<F, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
+  if (rc != HCA_OK) return true;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeCooperative;
   attr[0].val.cooperative = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sms);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem_bytes<F, NB, kWidth>(units));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, moe_layer_kernel<F, NB, kWidth>, p, w, shape));
+  rc = cuda_status(cudaLaunchKernelEx(&cfg, moe_layer_kernel<F, NB, kWidth>, p, w, shape));
+  return true;
 }
 
 }  // namespace moe
@@ -378,10 +399,11 @@ int launch(const MoePass& p, const MoeWeights& w, int units, cudaStream_t s) {
 template <int F>
 int moe_experts_pass(const MoePass& p, const MoeWeights& w, cudaStream_t s) {
   // Columns of an entry: as many as an expert may get and shared memory holds.
-  const int units = WTraits<F>::units(std::max(p.hidden, std::max(p.inner, p.shared_inner)));
-  if (p.tokens > 8 && moe::smem_bytes<F, 2, 8>(units) <= moe::kSmem) return moe::launch<F, 2, 8>(p, w, units, s);
-  if (p.tokens > 2 && moe::smem_bytes<F, 1, 8>(units) <= moe::kSmem) return moe::launch<F, 1, 8>(p, w, units, s);
-  if (moe::smem_bytes<F, 1, 2>(units) <= moe::kSmem) return moe::launch<F, 1, 2>(p, w, units, s);
+  int rc = HCA_OK;
+  if (p.tokens > 8 && moe::launch<F, 2, 8>(p, w, s, rc)) return rc;
+  if (p.tokens > 4 && moe::launch<F, 1, 8>(p, w, s, rc)) return rc;
+  if (p.tokens > 2 && moe::launch<F, 1, 4>(p, w, s, rc)) return rc;
+  if (moe::launch<F, 1, 2>(p, w, s, rc)) return rc;
   return HCA_E_UNSUPPORTED;
 }
 

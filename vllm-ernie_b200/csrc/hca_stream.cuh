@@ -14,10 +14,19 @@
 // once in the order in which the lanes use them.
 //
 // A "unit" is the piece of a row that the four lanes of a fragment row hold
-// at a time: 32 bf16, 64 e4m3 (16 bytes a lane in one load) or 128 4-bit
-// codes (16 bytes a lane; one load, or two or four for groups of 64 and 32,
-// so that each load stays inside a group).  Sums are held in 32 bits; group
-// and block scales multiply the 32-bit sums of their own groups.
+// at a time, 16 bytes a lane in one load: 32 bf16, 64 e4m3 or 128 4-bit codes.
+// (A load costs L1 a cycle for each of its eight rows whatever its width, so
+// narrower ones would cap the rate.)  A warp keeps four units on their way in
+// registers, across the ends of tiles.  Rings in shared memory, filled by TMA
+// boxes or asynchronous copies, were slower (3.7 TB/s where this came to 4.8):
+// each unit then starts with a wait and a read that nothing overlaps.  So were
+// loops that keep one copy of the code for tiles' ends: where paths meet the
+// compiler has to wait for every load under way.  A product may only sum
+// over one group of codes; with groups of 64 or 32 the four lanes exchange
+// words first.  Sums are held in 32 bits; group and block scales multiply the
+// 32-bit sums of their own groups.  The 4-bit scales and zero points of a
+// warp's share of a tile come into shared memory a tile ahead, in runs along the
+// rows: loaded unit by unit they cost L1 more cycles than the codes.
 //
 // No code is converted.  The smallest floats of a 16-bit type are evenly
 // spaced: bits 0..7 of a bf16 (0..10 of an fp16) with nothing above them are
@@ -50,12 +59,11 @@ template <int F>
 struct WTraits {
   static constexpr bool kIs4 = F >= kW4G32;
   static constexpr int kUnitK = F == kWBf16 ? 32 : F == kWFp8 ? 64 : 128;
-  // loads of a row for a unit, each inside one group
-  static constexpr int kSub = F == kW4G32 ? 4 : F == kW4G64 ? 2 : 1;
-  static constexpr int kWords = 4 / kSub;              // 32-bit words of a load and lane
-  static constexpr int kPieces = kUnitK / 32;          // 16-byte activation pieces of a lane and column
-  static constexpr int kGroupK = kUnitK / kSub;        // reduction length of a load
-  static constexpr int kLaneK = kGroupK / 4;           // and of a lane's share of it
+  static constexpr int kSub = F == kW4G32 ? 4 : F == kW4G64 ? 2 : 1;  // groups of a unit
+  static constexpr int kPieces = kUnitK / 32;    // 16-byte activation pieces of a lane and column
+  static constexpr int kGroupK = kUnitK / kSub;  // reduction length of a group
+  // k may end inside a unit
+  static constexpr bool kRagged = F == kWFp8 || F == kW4G32 || F == kW4G64;
   __host__ __device__ static constexpr int64_t row_bytes(int64_t k) {
     return F == kWBf16 ? 2 * k : F == kWFp8 ? k : k / 2;
   }
@@ -78,6 +86,11 @@ struct MmaType<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+  // both halves times a power of two, exactly
+  static __device__ __forceinline__ uint32_t times(uint32_t v, float f) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&v), __float2bfloat162_rn(f));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
   static __device__ __forceinline__ float to_float(uint16_t v) { return bf16_bits_to_float(v); }
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
@@ -110,84 +123,54 @@ struct Scaling {
   static constexpr float kOut = F == kWBf16 ? 1.0f : kHalf ? 0x1p24f : F == kWFp8 ? 0x1p40f : 0x1p53f;
 };
 
-// Weights are read once: past L1.
-template <int kWords>
-__device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p) {
-  if constexpr (kWords == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "l"(p));
-  } else if constexpr (kWords == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0,%1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-  } else {
-    // 16 bytes of a row at a time: the other half of the sector is the next load's
-    asm volatile("ld.global.nc.L2::256B.u32 %0, [%1];\n" : "=r"(w[0]) : "l"(p));
+// The words of a unit by group: on return lane c of the four holds words of
+// group i alone in w[i * 4 / kSub ..].  With groups of 32 that is a transpose
+// of the four lanes' words, with groups of 64 an exchange of two.
+template <int F>
+__device__ __forceinline__ void by_group(uint32_t (&w)[4]) {
+  const int c = threadIdx.x & 3;
+  if constexpr (F == kW4G64) {
+    const bool up = c & 2;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t v = __shfl_xor_sync(0xffffffffu, up ? w[i] : w[i + 2], 2);
+      if (up) w[i] = v; else w[i + 2] = v;
+    }
+  } else if constexpr (F == kW4G32) {
+    const bool b0 = c & 1, b1 = c & 2;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const uint32_t v = __shfl_xor_sync(0xffffffffu, b0 ? w[i] : w[i + 1], 1);
+      if (b0) w[i] = v; else w[i + 1] = v;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t v = __shfl_xor_sync(0xffffffffu, b1 ? w[i] : w[i + 2], 2);
+      if (b1) w[i] = v; else w[i + 2] = v;
+    }
   }
 }
 
-// A unit of two rows on its way from memory.
-template <int F>
-struct WStep {
-  static constexpr int kScales = F == kWBf16 ? 0 : WTraits<F>::kSub;
-  uint32_t w[2][4];
-  uint32_t s[2][kScales > 0 ? kScales : 1];  // bits of the scales
-  uint32_t z[2][WTraits<F>::kIs4 ? kScales : 1];
-};
-
-// A lane's two rows of a tile (fragment rows lane / 4 and lane / 4 + 8), read
-// unit after unit.  Lanes whose share of a row's last unit lies past its end
-// read its last bytes again; the activations there are zeros.
-template <int F>
-struct WCursor {
-  using W = WTraits<F>;
-  const uint8_t* data[2];
-  const void* scale[2];    // 4-bit: 16-bit scales of the row's groups; e4m3: fp32 scales of its blocks
-  const uint8_t* zero[2];  // zero points of the row's groups, or null
-  int unit;
-
-  // kRagged: k may end inside a unit (never for bf16 and groups of 128)
-  static constexpr bool kRagged = F == kWFp8 || F == kW4G32 || F == kW4G64;
-
-  // data[] of lane c starts c * 4 kWords bytes into the row
-  __device__ __forceinline__ void load(WStep<F>& st, int k) {
-    constexpr int kBytes = static_cast<int>(W::row_bytes(W::kUnitK));
-#pragma unroll
-    for (int i = 0; i < W::kSub; ++i) {
-      int off = unit * kBytes + i * 16 * W::kWords;
-      if (kRagged) off = min(off, static_cast<int>(W::row_bytes(k)) - 4 * W::kWords * (1 + (static_cast<int>(threadIdx.x) & 3)));
-#pragma unroll
-      for (int r = 0; r < 2; ++r) load_words<W::kWords>(&st.w[r][i * W::kWords], data[r] + off);
-    }
-    if constexpr (W::kIs4) {
-#pragma unroll
-      for (int i = 0; i < W::kSub; ++i) {
-        int g = unit * W::kSub + i;
-        if (kRagged) g = min(g, k / W::kGroupK - 1);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          st.s[r][i] = __ldg(static_cast<const uint16_t*>(scale[r]) + g);
-          st.z[r][i] = 8;
-          if (zero[r] != nullptr) st.z[r][i] = __ldg(zero[r] + g);
-        }
-      }
-    } else if constexpr (F == kWFp8) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        st.s[r][0] = __float_as_uint(__ldg(static_cast<const float*>(scale[r]) + unit / 2));  // blocks of 128
-    }
-    ++unit;
-  }
-};
-
 // Place of the 16-byte piece that holds column col's activations k .. k + 7
 // (k a multiple of 8) among the pieces of a block of columns: the pieces of a
-// unit follow each other, each 4 kWidth lanes wide.
+// unit follow each other, each 4 kWidth lanes wide.  The lanes of a piece are
+// swapped around by `piece_swap`, so that eight threads that lay out
+// consecutive activations write to eight different bank groups.
+template <int F>
+__device__ __forceinline__ int piece_swap(int u, int j) {
+  return F == kWBf16 ? 4 * (u & 1) : F == kW4G128 ? 2 * j : 4 * (j & 1);
+}
 template <int F, int kWidth>
 __device__ __forceinline__ int piece_index(int k, int col) {
   using W = WTraits<F>;
-  const int u = k / W::kUnitK, i = k % W::kUnitK / W::kGroupK, c = k % W::kGroupK / W::kLaneK;
-  const int j = i * (W::kLaneK / 8) + k % W::kLaneK / 8;
-  return ((u * W::kPieces + j) * kWidth + col) * 4 + c;
+  const int u = k / W::kUnitK, r = k % W::kUnitK;
+  int c, j;
+  if constexpr (F == kWBf16) c = r / 8, j = 0;
+  else if constexpr (F == kWFp8) c = r / 16, j = r / 8 % 2;
+  else if constexpr (F == kW4G128) c = r / 32, j = r / 8 % 4;
+  else if constexpr (F == kW4G64) c = r / 32 % 2 + r / 16 % 2 * 2, j = r / 64 * 2 + r / 8 % 2;
+  else c = r / 8 % 4, j = r / 32;
+  return (u * W::kPieces + j) * kWidth * 4 + ((col * 4 + c) ^ piece_swap<F>(u, j));
 }
 
 // Eight consecutive activations in a piece's order, that in which weights come
@@ -196,11 +179,7 @@ template <int F, typename T>
 __device__ __forceinline__ uint4 piece_order(uint4 v) {
   using M = MmaType<T>;
   constexpr float kX = Scaling<F, T>::kX;
-  if constexpr (kX != 1.0f) {
-    const float2 a = M::unpack(v.x), b = M::unpack(v.y), c = M::unpack(v.z), d = M::unpack(v.w);
-    v = make_uint4(M::pack(a.x * kX, a.y * kX), M::pack(b.x * kX, b.y * kX), M::pack(c.x * kX, c.y * kX),
-                   M::pack(d.x * kX, d.y * kX));
-  }
+  if constexpr (kX != 1.0f) v = make_uint4(M::times(v.x, kX), M::times(v.y, kX), M::times(v.z, kX), M::times(v.w, kX));
   if constexpr (WTraits<F>::kIs4)
     return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                       __byte_perm(v.y, v.w, 0x7632));
@@ -209,6 +188,88 @@ __device__ __forceinline__ uint4 piece_order(uint4 v) {
                       __byte_perm(v.z, v.w, 0x7632));
   return v;
 }
+
+// The warps that share a tile: warp `index` of `warps`, group `id` of the
+// block.  They take the tile's units in even runs and add their sums here.
+struct TileGroup {
+  int warps, index, id;
+
+  __device__ __forceinline__ explicit TileGroup(int warps_)
+      : warps(warps_), index((threadIdx.x >> 5) % warps_), id((threadIdx.x >> 5) / warps_) {}
+  __device__ __forceinline__ int first_unit(int units) const { return units * index / warps; }
+  __device__ __forceinline__ int end_unit(int units) const { return units * (index + 1) / warps; }
+  __device__ __forceinline__ int threads() const { return warps * 32; }
+  __device__ __forceinline__ int thread() const { return index * 32 + (threadIdx.x & 31); }
+
+  // Waits for the whole group; barriers 1..15 are the groups'.
+  __device__ __forceinline__ void sync() const {
+    if (warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + id), "r"(warps * 32) : "memory");
+  }
+};
+
+// Where a tile row's scales and zero points are (4-bit only): the addresses of
+// the row's first, and the ends of the whole arrays.
+struct WScales {
+  const uint8_t *scale, *scale_end;
+  const uint8_t *zero, *zero_end;  // null: 8 everywhere
+};
+
+// Scales and zero points of a warp's share of a tile, in shared memory, two
+// tiles in turn.  If every row's share begins and ends on 16 bytes (wide), it
+// is copied in pieces of 16 (zero points 8); else whole words around it are,
+// and it starts 0..3 bytes into the first.
+template <int F>
+struct ScaleTile {
+  using W = WTraits<F>;
+  uint8_t* base;  // this warp's: [2][16 rows][scales, zero points]
+  int pitch, zero_at;
+  bool wide;
+
+  // bytes of a row: n scales and n zero points, each with room for words'
+  // edges; an odd number of 16 bytes, so that eight rows start in different banks
+  __host__ __device__ static int zero_offset(int n) { return (2 * n + 15) / 16 * 16 + (n % 8 ? 16 : 0); }
+  __host__ __device__ static int row_pitch(int n, bool zeros) {
+    return ((zero_offset(n) + (zeros ? n + 8 : 0) + 15) / 16 | 1) * 16;
+  }
+  // most groups of a warp's share
+  __host__ __device__ static int share(int units, int warps) { return (units + warps - 1) / warps * W::kSub; }
+  __host__ __device__ static int64_t bytes(int units, bool zeros, int group_warps, int block_warps) {
+    return W::kIs4 ? 32ll * block_warps * row_pitch(share(units, group_warps), zeros) : 0;
+  }
+
+  __device__ __forceinline__ void init(uint8_t* smem, int units, bool zeros, int warps, int groups, int g0, int g1) {
+    const int n = share(units, warps);
+    zero_at = zero_offset(n), pitch = row_pitch(n, zeros);
+    base = smem + (threadIdx.x >> 5) * 32 * pitch;
+    wide = ((groups | g0 | g1 | n) & 7) == 0;
+  }
+  __device__ __forceinline__ uint8_t* row(int i, int r) const { return base + ((i & 1) * 16 + r) * pitch; }
+  // Starts the copy of groups [g0, g1) of the lane's row of tile `i`: lanes l
+  // and l + 16 row l.
+  __device__ __forceinline__ void fetch(int i, const WScales& from, int g0, int g1) const {
+    const int lane = threadIdx.x & 31, half = lane >> 4;
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(row(i, lane & 15)));
+    if (wide) {
+      for (int g = g0 + 8 * half; g < g1; g += 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 2 * (g - g0)), "l"(from.scale + 2 * g) : "memory");
+        if (from.zero != nullptr)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + zero_at + g - g0), "l"(from.zero + g) : "memory");
+      }
+    } else {
+      copy(to, from.scale + 2 * g0, from.scale + 2 * g1, from.scale_end, half);
+      if (from.zero != nullptr) copy(to + zero_at, from.zero + g0, from.zero + g1, from.zero_end, half);
+    }
+  }
+  static __device__ __forceinline__ void copy(uint32_t to, const uint8_t* from, const uint8_t* until, const uint8_t* end, int first) {
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t{3}) + 4 * first;
+    to += 4 * first;
+    for (; p < until; p += 8, to += 8) {
+      const int n = static_cast<int>(min(static_cast<int64_t>(4), static_cast<int64_t>(end - p)));  // not past the array
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to), "l"(p), "r"(n) : "memory");
+    }
+  }
+};
 
 // Activations of NB blocks of columns in shared memory, in piece order, with
 // their group sums.  A block has 8 columns, of which kWidth are stored.
@@ -237,7 +298,7 @@ struct XTile {
   __device__ __forceinline__ void stage(int k, int columns, int live, Row row) {
     const int padded = units * W::kUnitK;
     // several columns' loads under way at a time
-    constexpr int kAhead = kWidth < 4 ? kWidth : 4;
+    constexpr int kAhead = kWidth;
     for (int c0 = 0; c0 < live * kWidth; c0 += kAhead) {
       const T* p[kAhead];
 #pragma unroll
@@ -263,7 +324,7 @@ struct XTile {
         if (lane < kWidth * 4) {
 #pragma unroll
           for (int q = 0; q < kEach; ++q) {
-            const uint4 x = pieces[(g * kEach + q) * kWidth * 4 + lane];
+            const uint4 x = pieces[(g * kEach + q) * kWidth * 4 + (lane ^ piece_swap<F>(0, g % W::kSub * kEach + q))];
             const float2 a = MmaType<T>::unpack(x.x), b = MmaType<T>::unpack(x.y), c = MmaType<T>::unpack(x.z),
                          d = MmaType<T>::unpack(x.w);
             v += ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
@@ -280,13 +341,15 @@ struct XTile {
   }
 
   // acc[b] += the step's rows times the columns of block b < NBL, over unit u.
-  template <int NBL>
-  __device__ __forceinline__ void consume(float (&acc)[NB][4], const WStep<F>& st, int u) const {
+  // w: the lane's shares of fragment rows lane / 4 and lane / 4 + 8;
+  // scales(i, s, z) gives these rows' scale and zero point of the unit's group i.
+  template <int NBL, typename Scales>
+  __device__ __forceinline__ void consume(float (&acc)[NB][4], uint32_t (&w)[2][4], int u, Scales scales) const {
     using M = MmaType<T>;
     const int lane = threadIdx.x & 31;
-    const uint4* at = pieces + u * kUnitPieces + lane;
+    const uint4* at = pieces + u * kUnitPieces;
     auto piece = [&](int b, int j) -> uint4 {
-      const uint4* p = at + b * units * kUnitPieces + j * kWidth * 4;
+      const uint4* p = at + b * units * kUnitPieces + j * kWidth * 4 + (lane ^ piece_swap<F>(u, j));
       if (kWidth == 8) return *p;
       return lane < kWidth * 4 ? *p : make_uint4(0, 0, 0, 0);
     };
@@ -294,10 +357,14 @@ struct XTile {
 #pragma unroll
       for (int b = 0; b < NBL; ++b) {
         const uint4 x = piece(b, 0);
-        M::mma(acc[b], st.w[0][0], st.w[1][0], st.w[0][1], st.w[1][1], x.x, x.y);
-        M::mma(acc[b], st.w[0][2], st.w[1][2], st.w[0][3], st.w[1][3], x.z, x.w);
+        M::mma(acc[b], w[0][0], w[1][0], w[0][1], w[1][1], x.x, x.y);
+        M::mma(acc[b], w[0][2], w[1][2], w[0][3], w[1][3], x.z, x.w);
       }
     } else {
+      if constexpr (W::kIs4) {
+        by_group<F>(w[0]);
+        by_group<F>(w[1]);
+      }
 #pragma unroll
       for (int i = 0; i < W::kSub; ++i) {
         float part[NBL][4] = {}, high[NBL][4] = {};
@@ -308,17 +375,17 @@ struct XTile {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             if constexpr (W::kIs4) {
-              const uint32_t w = st.w[r][j], v = w >> 8;
-              a[r][0] = w & 0x000f000fu;
+              const uint32_t lo = w[r][j], v = lo >> 8;
+              a[r][0] = lo & 0x000f000fu;
               a[r][1] = v & 0x000f000fu;
-              a[r][2] = w & 0x00f000f0u;
+              a[r][2] = lo & 0x00f000f0u;
               a[r][3] = v & 0x00f000f0u;
             } else {
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
-                const uint32_t w = st.w[r][2 * j + n];
-                a[r][2 * n] = ((w << 4) & 0x07f007f0u) | ((w << 8) & 0x80008000u);
-                a[r][2 * n + 1] = ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u);
+                const uint32_t v = w[r][2 * j + n];
+                a[r][2 * n] = ((v << 4) & 0x07f007f0u) | ((v << 8) & 0x80008000u);
+                a[r][2 * n + 1] = ((v >> 4) & 0x07f007f0u) | (v & 0x80008000u);
               }
             }
           }
@@ -329,10 +396,8 @@ struct XTile {
             M::mma(high[b], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
           }
         }
-        float s[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          s[r] = W::kIs4 ? M::to_float(static_cast<uint16_t>(st.s[r][i])) : __uint_as_float(st.s[r][i]);
+        float s[2], z[2];
+        scales(i, s, z);
 #pragma unroll
         for (int b = 0; b < NBL; ++b) {
 #pragma unroll
@@ -341,9 +406,8 @@ struct XTile {
             const float2 x = *reinterpret_cast<const float2*>(sums + ((b * units + u) * W::kSub + i) * 8 + 2 * (lane & 3));
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const float z = -static_cast<float>(st.z[r][i]);
-              part[b][2 * r] = fmaf(z, x.x, part[b][2 * r]);
-              part[b][2 * r + 1] = fmaf(z, x.y, part[b][2 * r + 1]);
+              part[b][2 * r] = fmaf(-z[r], x.x, part[b][2 * r]);
+              part[b][2 * r + 1] = fmaf(-z[r], x.y, part[b][2 * r + 1]);
             }
           }
 #pragma unroll
@@ -351,25 +415,6 @@ struct XTile {
         }
       }
     }
-  }
-};
-
-// The warps that share a tile: warp `index` of `warps`, group `id` of the
-// block.  They take the tile's units in even runs and add their sums here.
-struct TileGroup {
-  int warps, index, id;
-
-  __device__ __forceinline__ explicit TileGroup(int warps_)
-      : warps(warps_), index((threadIdx.x >> 5) % warps_), id((threadIdx.x >> 5) / warps_) {}
-  __device__ __forceinline__ int first_unit(int units) const { return units * index / warps; }
-  __device__ __forceinline__ int end_unit(int units) const { return units * (index + 1) / warps; }
-  __device__ __forceinline__ int threads() const { return warps * 32; }
-  __device__ __forceinline__ int thread() const { return index * 32 + (threadIdx.x & 31); }
-
-  // Waits for the whole group; barriers 1..15 are the groups'.
-  __device__ __forceinline__ void sync() const {
-    if (warps == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + id), "r"(warps * 32) : "memory");
   }
 };
 
@@ -409,49 +454,133 @@ struct TileSums {
   }
 };
 
-// Units of a run of tiles on their way: kDepth of them, across the ends of
-// tiles.  rows(cur, i) points the cursor at the rows of the group's i-th tile.
-template <int F>
-struct TileRing {
-  // groups of 32 bring eight scales and zero points a unit
-  static constexpr int kDepth = F == kW4G32 ? 3 : 4;
-  WStep<F> st[kDepth];
-  WCursor<F> cur;
-  int k, u0, u1, next, count;
+// Weights are read once: past L1, a few units ahead into L2.
+__device__ __forceinline__ void load_weights(uint32_t (&w)[4], const uint8_t* p) {
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "l"(p));
+}
 
-  template <typename Rows>
-  __device__ __forceinline__ void load(WStep<F>& s, Rows& rows) {
+// The lane's two rows of a tile (fragment rows lane / 4 and lane / 4 + 8) and
+// the unit of them to load next.  data[] starts 16 (lane % 4) bytes into the row.
+template <int F>
+struct WCursor {
+  const uint8_t* data[2];
+  const float* scale[2];  // e4m3: of the row's blocks
+  int unit;
+};
+
+// Units of a run of tiles on their way, kDepth of them, across the ends of
+// tiles.  `source` knows the tiles: source.rows(cur, i) points the cursor at
+// the rows of the group's i-th tile, source.scales(i, row) tells where the
+// scales of a row of it are and source.here the same for the tile now consumed,
+// source.zeros whether there are zero points (4-bit only).  Each is asked for
+// the tiles in order.
+template <int F, typename T>
+struct TileRing {
+  using W = WTraits<F>;
+  static constexpr int kDepth = 4;
+  struct Step {
+    uint32_t w[2][4];
+    float s[2];  // e4m3
+  } st[kDepth];
+  WCursor<F> cur;
+  ScaleTile<F> sc;
+  int k, u0, u1, next, count, g0, g1;
+
+  // Lanes whose share of a row's last unit lies past its end read its last
+  // bytes again; the activations there are zeros.
+  template <typename Source>
+  __device__ __forceinline__ void load(Step& s, Source& source) {
     if (next >= count) return;
-    cur.load(s, k);
-    if (cur.unit == u1) {
-      ++next;
-      if (next < count) rows(cur, next);
+    int off = cur.unit * 64;
+    if (W::kRagged) off = min(off, static_cast<int>(W::row_bytes(k)) - 16 * (1 + (static_cast<int>(threadIdx.x) & 3)));
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      load_weights(s.w[r], cur.data[r] + off);
+      if (F == kWFp8) s.s[r] = __ldg(cur.scale[r] + cur.unit / 2);  // blocks of 128
+    }
+    if (++cur.unit == u1) {
       cur.unit = u0;
+      if (++next < count) source.rows(cur, next);
     }
   }
-  // Starts the loads of `count` tiles of rows of k, this warp's share of each.
-  template <typename Rows>
-  __device__ __forceinline__ void start(int k_, const TileGroup& g, int count_, Rows rows) {
-    const int units = WTraits<F>::units(k_);
+  template <typename Source>
+  __device__ __forceinline__ void fetch_scales(int i, Source& source) const {
+    if constexpr (W::kIs4) {
+      if (i < count) sc.fetch(i, source.scales(i, threadIdx.x & 15), g0, g1);
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
+  }
+  // Starts the loads of `count` tiles of rows of k, this warp's share of each;
+  // `smem` is for the scales, of ScaleTile::bytes(units, ...) at most.
+  template <typename Source>
+  __device__ __forceinline__ void start(int k_, const TileGroup& g, int count_, uint8_t* smem, Source& source) {
+    const int units = W::units(k_);
     k = k_, u0 = g.first_unit(units), u1 = g.end_unit(units), next = 0, count = count_;
     cur.unit = u0;
-    if (count > 0) rows(cur, 0);
+    if (count > 0) source.rows(cur, 0);
 #pragma unroll
-    for (int d = 0; d < kDepth; ++d) load(st[d], rows);
+    for (int d = 0; d < kDepth; ++d) load(st[d], source);
+    if constexpr (W::kIs4) {
+      g0 = u0 * W::kSub, g1 = min(u1 * W::kSub, k / W::kGroupK);
+      sc.init(smem, units, source.zeros(), g.warps, k / W::kGroupK, g0, g1);
+      __syncwarp();  // the last run's scales have been read
+      fetch_scales(0, source);
+      fetch_scales(1, source);
+    }
   }
   // Consumes them; finish(i, sums) for each tile, in order.
-  template <int NBL, typename X, typename Sums, int NB, typename Rows, typename Finish>
-  __device__ __forceinline__ void run(const X& xt, const TileGroup& g, Sums& ts, float (&acc)[NB][4], Rows rows, Finish finish) {
+  template <int NBL, typename X, typename Sums, int NB, typename Source, typename Finish>
+  __device__ __forceinline__ void run(const X& xt, const TileGroup& g, Sums& ts, float (&acc)[NB][4], Source& source, Finish finish) {
     int u = u0, i = 0;
+    const uint8_t *srow[2], *zrow[2];  // of the lane's rows, at group 0
+    auto begin_tile = [&]() {
+      if constexpr (W::kIs4) {
+        asm volatile("cp.async.wait_group 1;\n" ::: "memory");  // all but the next tile's
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = ((threadIdx.x & 31) >> 2) + 8 * r;
+          srow[r] = sc.row(i, row) - 2 * g0;
+          zrow[r] = sc.row(i, row) + sc.zero_at - g0;
+          if (!sc.wide) {
+            const WScales from = source.here(i, row);
+            srow[r] += reinterpret_cast<uintptr_t>(from.scale + 2 * g0) & 3;
+            zrow[r] += reinterpret_cast<uintptr_t>(from.zero + g0) & 3;
+          }
+        }
+      }
+    };
+    const bool zeros = W::kIs4 && source.zeros();
+    auto scales = [&](int d, int j, float (&s)[2], float (&z)[2]) {
+      if constexpr (W::kIs4) {
+        const int n = u * W::kSub + j;
+        const bool in = !W::kRagged || n < g1;  // no group: x is zero there
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          s[r] = in ? MmaType<T>::to_float(*reinterpret_cast<const uint16_t*>(srow[r] + 2 * n)) : 0.0f;
+          z[r] = zeros ? static_cast<float>(zrow[r][n]) : 8.0f;
+        }
+      } else {
+        s[0] = st[d].s[0], s[1] = st[d].s[1];
+      }
+    };
+    if (count > 0) begin_tile();
     while (i < count) {
 #pragma unroll
       for (int d = 0; d < kDepth; ++d) {
-        xt.template consume<NBL>(acc, st[d], u);
-        load(st[d], rows);
+        xt.template consume<NBL>(acc, st[d].w, u, [&](int j, float (&s)[2], float (&z)[2]) { scales(d, j, s, z); });
+        load(st[d], source);
         if (++u < u1) continue;
+        if constexpr (W::kIs4) {
+          __syncwarp();  // this tile's scales have been read
+          fetch_scales(i + 2, source);
+        }
         finish(i, ts.join(acc, g));
         u = u0;
         if (++i >= count) break;
+        begin_tile();
       }
     }
   }

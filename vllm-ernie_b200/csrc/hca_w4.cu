@@ -30,40 +30,54 @@ struct W4Args {
   int group_warps;  // warps that share a tile
 };
 
+// The tiles of a group of warps: first, first + stride, ...
+template <int F, typename T>
+struct W4Tiles {
+  using W = WTraits<F>;
+  const W4Args& a;
+  int first, stride, groups;
+
+  __device__ __forceinline__ int64_t row(int i, int r) const {
+    return min((first + i * stride) * 16 + r, a.n - 1);  // rows past the end are read again, not stored
+  }
+  __device__ __forceinline__ void rows(WCursor<F>& cur, int i) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) cur.data[r] = a.q + (lane & 3) * 16 + row(i, (lane >> 2) + 8 * r) * W::row_bytes(a.k);
+  }
+  __device__ __forceinline__ bool zeros() const { return a.zeros != nullptr; }
+  __device__ __forceinline__ WScales here(int i, int r) const {
+    const int64_t at = row(i, r) * groups, all = static_cast<int64_t>(a.n) * groups;
+    const uint8_t* s = static_cast<const uint8_t*>(a.scales);
+    return {s + 2 * at, s + 2 * all, a.zeros == nullptr ? nullptr : a.zeros + at, a.zeros + all};
+  }
+  __device__ __forceinline__ WScales scales(int i, int r) const { return here(i, r); }
+};
+
 template <int F, typename T, int NB, int kWidth>
 __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   using W = WTraits<F>;
   using X = XTile<F, T, NB, kWidth>;
   extern __shared__ __align__(16) uint8_t smem[];
-  const int lane = threadIdx.x & 31;
   const TileGroup g(a.group_warps);
-  const int units = W::units(a.k), groups = a.k / W::kGroupK;
+  const int units = W::units(a.k);
   X xt(smem, units);
   TileSums<NB> ts(smem + X::bytes(units));
-  const int tiles = (a.n + 15) / 16, per_cta = kWarps / g.warps, stride = gridDim.x * per_cta;
+  const int tiles = (a.n + 15) / 16, per_cta = kWarps / g.warps;
   const int t0 = blockIdx.y * X::kColumns;
   const int columns = min(X::kColumns, a.tokens - t0), live = (columns + kWidth - 1) / kWidth;
-  const int first = blockIdx.x * per_cta + g.id;
+  W4Tiles<F, T> src{a, static_cast<int>(blockIdx.x) * per_cta + g.id, static_cast<int>(gridDim.x) * per_cta, a.k / W::kGroupK};
 
   pdl_wait_and_release();
-  auto rows = [&](WCursor<F>& cur, int i) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      // rows past the end are read again, not stored
-      const int64_t row = min((first + i * stride) * 16 + (lane >> 2) + 8 * r, a.n - 1);
-      cur.data[r] = a.q + row * W::row_bytes(a.k) + (lane & 3) * 4 * W::kWords;
-      cur.scale[r] = static_cast<const T*>(a.scales) + row * groups;
-      cur.zero[r] = a.zeros == nullptr ? nullptr : a.zeros + row * groups;
-    }
-  };
-  TileRing<F> ring;
-  ring.start(a.k, g, first < tiles ? (tiles - first + stride - 1) / stride : 0, rows);
+  TileRing<F, T> ring;
+  ring.start(a.k, g, src.first < tiles ? (tiles - src.first + src.stride - 1) / src.stride : 0,
+             smem + X::bytes(units) + TileSums<NB>::bytes(kWarps), src);
   const T* x = static_cast<const T*>(a.x) + t0 * a.x_stride;
   xt.stage(a.k, columns, live, [&](int col) { return x + col * a.x_stride; });
 
   float acc[NB][4] = {};
   auto finish = [&](int i, const float* sums) {
-    const int row0 = (first + i * stride) * 16;
+    const int row0 = (src.first + i * src.stride) * 16;
     for (int j = g.thread(); j < live * 128; j += g.threads()) {
       const int row = row0 + (j & 15), block = j >> 7, col = (j >> 4) & 7, t = block * kWidth + col;
       if (row < a.n && col < kWidth && t < columns)
@@ -71,42 +85,46 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
             MmaType<T>::from_float(TileSums<NB>::sum(sums, g, j & 15, block, col) * Scaling<F, T>::kOut);
     }
   };
-  if (NB > 1 && live == 1) ring.template run<1>(xt, g, ts, acc, rows, finish);
-  else ring.template run<NB>(xt, g, ts, acc, rows, finish);
+  if (NB > 1 && live == 1) ring.template run<1>(xt, g, ts, acc, src, finish);
+  else ring.template run<NB>(xt, g, ts, acc, src, finish);
 }
 
+// Launches with NB blocks of kWidth columns if shared memory holds them.
 template <int F, typename T, int NB, int kWidth>
-constexpr int64_t smem_bytes(int units) {
-  return XTile<F, T, NB, kWidth>::bytes(units) + TileSums<NB>::bytes(kWarps);
-}
-
-template <int F, typename T, int NB, int kWidth>
-int launch(W4Args a, cudaStream_t s) {
+bool launch(W4Args a, cudaStream_t s, int& rc) {
   const int units = WTraits<F>::units(a.k), tiles = cdiv(a.n, 16), sms = device_sm_count();
-  // Warps to a tile: as few as leave every SM's groups four tiles each, but
-  // at least one unit a warp.  Few warps mean long runs between reductions,
-  // many that a short matrix still fills the machine.
+  const int64_t columns = XTile<F, T, NB, kWidth>::bytes(units) + TileSums<NB>::bytes(kWarps);
+  auto scales = [&](int warps) { return ScaleTile<F>::bytes(units, a.zeros != nullptr, warps, kWarps); };
+  // Warps to a tile: as few as leave every SM's groups four tiles each and
+  // room for the scales, but at least four units a warp (one step of its
+  // ring), or one where the tiles are too few to fill the machine otherwise.
+  // Few warps mean long runs between reductions.
   a.group_warps = 1;
-  while (a.group_warps < kWarps && tiles < 4ll * sms * (kWarps / a.group_warps) && 2 * a.group_warps <= units)
+  while (a.group_warps < kWarps && 2 * a.group_warps <= units &&
+         (tiles < (units >= 8 * a.group_warps ? 4ll : 1ll) * sms * (kWarps / a.group_warps) ||
+          columns + scales(a.group_warps) > kSmem))
     a.group_warps *= 2;
-  const int per_cta = kWarps / a.group_warps;
+  const int64_t smem = columns + scales(a.group_warps);
+  if (smem > kSmem) return false;
   static bool done[kMaxDevices] = {};
-  if (set_func_attr_once(w4_linear_kernel<F, T, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem,
-                         done) != HCA_OK)
-    return HCA_E_CUDA;
-  return launch_pdl(w4_linear_kernel<F, T, NB, kWidth>,
-                    dim3(std::min(sms, cdiv(tiles, per_cta)), cdiv(a.tokens, NB * kWidth)), dim3(kWarps * 32),
-                    smem_bytes<F, T, NB, kWidth>(units), s, a);
+  rc = set_func_attr_once(w4_linear_kernel<F, T, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
+  if (rc == HCA_OK) {
+    rc = launch_pdl(w4_linear_kernel<F, T, NB, kWidth>,
+                    dim3(std::min(sms, cdiv(tiles, kWarps / a.group_warps)), cdiv(a.tokens, NB * kWidth)),
+                    dim3(kWarps * 32), static_cast<size_t>(smem), s, a);
+  }
+  return true;
 }
 
 template <int F, typename T>
-int by_rows(W4Args a, cudaStream_t s) {
-  const int units = WTraits<F>::units(a.k);
+int by_rows(const W4Args& a, cudaStream_t s) {
   // Columns of x a pass holds: as many as there are rows and shared memory
   // for; what is left takes further passes over the weights.
-  if (a.tokens > 8 && smem_bytes<F, T, 2, 8>(units) <= kSmem) return launch<F, T, 2, 8>(a, s);
-  if (a.tokens > 2 && smem_bytes<F, T, 1, 8>(units) <= kSmem) return launch<F, T, 1, 8>(a, s);
-  if (smem_bytes<F, T, 1, 2>(units) <= kSmem) return launch<F, T, 1, 2>(a, s);
+  int rc = HCA_OK;
+  if (a.tokens > 8 && launch<F, T, 2, 8>(a, s, rc)) return rc;
+  if (a.tokens > 4 && launch<F, T, 1, 8>(a, s, rc)) return rc;
+  if (a.tokens > 2 && launch<F, T, 1, 4>(a, s, rc)) return rc;
+  if (launch<F, T, 1, 2>(a, s, rc)) return rc;
   return HCA_E_UNSUPPORTED;
 }
 
@@ -131,8 +149,8 @@ extern "C" int hca_w4_linear(void* out, int64_t out_stride, const void* x, int64
   if (num_tokens == 0) return HCA_OK;
   HCA_CHECK_ARG(out && x && q && scales);
   HCA_CHECK_ARG(x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0);
-  HCA_CHECK_ARG(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 2 == 0 &&
-                reinterpret_cast<uintptr_t>(out) % 2 == 0);
+  HCA_CHECK_ARG(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0 &&
+                reinterpret_cast<uintptr_t>(zeros) % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 2 == 0);
   HCA_CHECK_ARG(num_tokens <= 65535 && n <= INT32_MAX - 16);  // grid columns hold at least one row of x
   W4Args a{out, out_stride, x, x_stride, q, scales, zeros, num_tokens, n, k, 1};
   cudaStream_t s = as_stream(stream);
