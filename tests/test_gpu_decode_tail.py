@@ -312,6 +312,8 @@ def _moe_bound(ref, size, terms):
     (8, 40, 8, 512, 128, 128),
     (9, 3, 3, 256, 384, 0),       # every expert gets every token: two blocks
     (31, 20, 5, 256, 128, 128),
+    (9, 2, 1, 256, 1536, 0),      # the products' warps grouped differently, groups without a tile
+    (1, 1, 1, 256, 512, 0),
     (64, 4, 3, 128, 256, 128),    # far more tokens an expert than columns
     (70, 33, 2, 256, 128, 0),     # a second pass with six tokens
 ])

@@ -127,11 +127,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     moe_choose_kernel(int32_t* ids, float* weights, const float* logits, int tokens, MoeRouting r) {
   pdl_wait_and_release();
   const int t = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= tokens) return;
-  int id;
-  float weight;
-  choose_experts(logits + static_cast<int64_t>(t) * r.experts, r, t, id, weight);
-  if (lane < r.top_k) ids[static_cast<int64_t>(t) * r.top_k + lane] = id, weights[static_cast<int64_t>(t) * r.top_k + lane] = weight;
+  choose_all(logits, r, t, tokens, tokens, [&](int t, int id, float weight) {
+    ids[static_cast<int64_t>(t) * r.top_k + lane] = id;
+    weights[static_cast<int64_t>(t) * r.top_k + lane] = weight;
+  });
 }
 
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

@@ -66,83 +66,93 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// One warp: the experts of token t.  Lane j < top_k returns with the j-th
-// choice and its weight (-1 and 0 for a token that takes no part).
-__device__ __forceinline__ void choose_experts(const float* logits, const MoeRouting& r, int t, int& id, float& weight) {
+// One warp: the experts of tokens t0, t0 + step, .. (NT of them, side by side,
+// since each choice waits for the one before; tokens from `tokens` on are left
+// out).  Lane j < top_k calls store(t, id, weight) for the j-th choice (-1 and 0
+// for a token that takes no part).  kPer: experts a lane holds.
+template <int kPer, int NT, typename Store>
+__device__ __forceinline__ void choose_experts(const float* logits, const MoeRouting& r, int t0, int step, int tokens, Store store) {
   const int lane = threadIdx.x & 31;
-  constexpr int kPer = kMoeExperts / 32;
-  const int per = (r.experts + 31) / 32;
-  float score[kPer];
-  uint32_t key[kPer];
+  float score[NT][kPer], bias[kPer];
+  uint32_t key[NT][kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    if (j >= per) break;
     const int e = lane + 32 * j;
-    score[j] = e < r.experts ? logits[e] : -INFINITY;
-  }
-  if (r.sigmoid) {
+    bias[j] = r.bias != nullptr && e < r.experts ? r.bias[e] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (j >= per) break;
-      score[j] = 1.0f / (1.0f + expf(-score[j]));
-    }
-  } else {
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (j >= per) break;
-      m = fmaxf(m, score[j]);
-    }
-    m = warp_max(m);
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (j >= per) break;
-      score[j] = expf(score[j] - m);
-      if (lane + 32 * j < r.experts) sum += score[j];
-    }
-    sum = warp_sum(sum);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (j >= per) break;
-      score[j] /= sum;
-    }
+    for (int n = 0; n < NT; ++n)
+      score[n][j] = e < r.experts ? logits[static_cast<int64_t>(min(t0 + n * step, tokens - 1)) * r.experts + e] : -INFINITY;
   }
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (j >= per) break;
-    const int e = lane + 32 * j;
-    // experts' keys are at least 1 (NaN's), absent and taken ones 0
-    key[j] = e < r.experts ? order_key(r.bias == nullptr ? score[j] : score[j] + r.bias[e]) + 1 : 0;
-  }
-  weight = 0.0f, id = -1;
-  for (int c = 0; c < r.top_k; ++c) {
-    uint32_t best = 0;
-    int at = 0;
-    float s = 0.0f;
+  for (int n = 0; n < NT; ++n) {
+    if (r.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (j >= per) break;
-      if (key[j] > best) best = key[j], at = j, s = score[j];
-    }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : ~0u);
-    const float v = __shfl_sync(0xffffffffu, s, e & 31);
-    if (lane == static_cast<int>(e & 31)) {
+      for (int j = 0; j < kPer; ++j) score[n][j] = __fdividef(1.0f, 1.0f + __expf(-score[n][j]));
+    } else {
+      float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) m = fmaxf(m, score[n][j]);
+      m = warp_max(m);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        if (j >= per) break;
-        if (j == static_cast<int>(e >> 5)) key[j] = 0;
+        score[n][j] = __expf(score[n][j] - m);
+        if (lane + 32 * j < r.experts) sum += score[n][j];
       }
+      sum = 1.0f / warp_sum(sum);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) score[n][j] *= sum;
     }
-    if (lane == c) weight = v, id = static_cast<int>(e);
+    // experts' keys are at least 1 (NaN's), absent and taken ones 0
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      key[n][j] = lane + 32 * j < r.experts ? order_key(r.bias == nullptr ? score[n][j] : score[n][j] + bias[j]) + 1 : 0;
   }
-  if (r.renormalize) {
-    const float sum = warp_sum(weight);
-    weight = sum == 0.0f ? 0.0f : weight / sum;  // every chosen score underflowed: no expert has weight
+  float weight[NT];
+  int id[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) weight[n] = 0.0f, id[n] = -1;
+#pragma unroll 1
+  for (int c = 0; c < r.top_k; ++c) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint32_t best = 0;
+      int at = 0;
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (key[n][j] > best) best = key[n][j], at = j, s = score[n][j];
+      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+      const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at * 32 + lane) : ~0u);
+      const float v = __shfl_sync(0xffffffffu, s, e & 31);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (static_cast<uint32_t>(lane + 32 * j) == e) key[n][j] = 0;
+      if (lane == c) weight[n] = v, id[n] = static_cast<int>(e);
+    }
   }
-  weight *= r.scale;
-  if (r.mask != nullptr && !r.mask[t]) id = -1, weight = 0.0f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int t = t0 + n * step;
+    float w = weight[n];
+    if (r.renormalize) {
+      const float sum = warp_sum(w);
+      w = sum == 0.0f ? 0.0f : w / sum;  // every chosen score underflowed: no expert has weight
+    }
+    const bool in = t < tokens && (r.mask == nullptr || r.mask[t]);
+    if (lane < r.top_k && t < tokens) store(t, in ? id[n] : -1, in ? w * r.scale : 0.0f);
+  }
+}
+
+// The experts of tokens t0, t0 + step, .. below `tokens`.
+template <typename Store>
+__device__ __forceinline__ void choose_all(const float* logits, const MoeRouting& r, int t0, int step, int tokens, Store store) {
+  if (r.experts > 128) {
+#pragma unroll 1
+    for (int t = t0; t < tokens; t += step) choose_experts<kMoeExperts / 32, 1>(logits, r, t, step, tokens, store);
+  } else {
+#pragma unroll 1
+    for (int t = t0; t < tokens; t += step) choose_experts<4, 1>(logits, r, t, step, tokens, store);
+  }
 }
 
 }  // namespace hca

@@ -32,65 +32,72 @@ constexpr int64_t kSmem = 208 * 1024;
 
 // Who computes what, made by every CTA from the ids (at most 1024 of them) in
 // shared memory.  A pair is t * top_k + j; the shared expert's are tokens *
-// top_k + t.  An entry is up to `columns` pairs of one expert, so that every
-// entry's weights cost one pass; entries are in the experts' order, the
-// shared expert (number `experts`) last, and pairs in theirs.
+// top_k + t.  An id that repeats in a token counts once, with the weights'
+// sum.  An entry is up to `columns` pairs of one expert, so that every entry's
+// weights cost one pass; entries are in the experts' order, the shared expert
+// (number `experts`) last, and pairs in the tokens'.
 template <int kColumns>
 struct Plan {
   static constexpr int kEntries = kMoeExperts + 1 + kMoePairs / kColumns;
-  int entries, routed;        // with and without the shared expert's
-  int16_t expert[kEntries];   // entry -> expert
+  int entries, routed;          // with and without the shared expert's
+  int16_t expert[kEntries];     // entry -> expert
   int16_t start[kEntries + 1];  // entry -> first pair
   int16_t pair[kMoePairs];
-  int16_t id[kMoePairs];        // pair -> expert, or -1
+  int16_t id[kMoePairs];  // pair -> expert, or -1
   float weight[kMoePairs];
-  int16_t rank[kMoePairs];      // pair -> place in its expert's list
-  int16_t list[kMoeExperts + 1];  // expert -> number of pairs, then first pair
+  uint64_t who[kMoeExperts + 1];  // expert -> its tokens
+  int16_t list[kMoeExperts + 1];  // expert -> first pair
 };
 
 template <int kColumns>
 __device__ __forceinline__ void build_plan(Plan<kColumns>& pl, const MoePass& p) {
   const int lane = threadIdx.x & 31, top_k = p.routing.top_k, experts = p.routing.experts;
   const int routed = p.tokens * top_k, n = routed + p.tokens;
+  const uint8_t* mask = p.routing.mask;
+#pragma unroll 1
+  for (int e = threadIdx.x; e <= experts; e += kThreads) pl.who[e] = 0;
   if (p.logits != nullptr) {
-    for (int t = threadIdx.x >> 5; t < p.tokens; t += kWarps) {
-      int id;
-      float weight;
-      choose_experts(p.logits + static_cast<int64_t>(t) * experts, p.routing, t, id, weight);
-      if (lane < top_k) pl.id[t * top_k + lane] = static_cast<int16_t>(id), pl.weight[t * top_k + lane] = weight;
-    }
+    choose_all(p.logits, p.routing, threadIdx.x >> 5, kWarps, p.tokens, [&](int t, int id, float weight) {
+      pl.id[t * top_k + lane] = static_cast<int16_t>(id);
+      pl.weight[t * top_k + lane] = weight;
+    });
   } else {
+#pragma unroll 1
     for (int i = threadIdx.x; i < routed; i += kThreads) {
-      const int e = p.routing.mask == nullptr || p.routing.mask[i / top_k] ? p.ids[i] : -1;
-      pl.id[i] = static_cast<int16_t>(e >= 0 && e < experts ? e : -1);
-      pl.weight[i] = p.weights[i];
+      const int t = i / top_k;
+      const int32_t* ids = p.ids + static_cast<int64_t>(t) * top_k;
+      const float* weights = p.weights + static_cast<int64_t>(t) * top_k;
+      const int j = i - t * top_k, e = ids[j];
+      bool in = e >= 0 && e < experts && (mask == nullptr || mask[t]);
+      float weight = 0.0f;
+#pragma unroll 1
+      for (int o = 0; o < top_k; ++o) {
+        if (ids[o] != e) continue;
+        if (o < j) in = false;
+        weight += weights[o];
+      }
+      pl.id[i] = static_cast<int16_t>(in ? e : -1);
+      pl.weight[i] = weight;
     }
   }
+#pragma unroll 1
   for (int t = threadIdx.x; t < p.tokens; t += kThreads) {
-    const bool in = p.shared_inner > 0 && (p.routing.mask == nullptr || p.routing.mask[t]);
+    const bool in = p.shared_inner > 0 && (mask == nullptr || mask[t]);
     pl.id[routed + t] = static_cast<int16_t>(in ? experts : -1);
     pl.weight[routed + t] = 1.0f;
   }
-  for (int e = threadIdx.x; e <= experts; e += kThreads) pl.list[e] = 0;
+  __syncthreads();
+  auto token = [&](int i) { return i < routed ? i / top_k : i - routed; };
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads)
+    if (pl.id[i] >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&pl.who[pl.id[i]]), 1ull << token(i));
   __syncthreads();
   if (threadIdx.x < 32) {
-    // 32 pairs at a time, so that the lists come out in order
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      const int e = i < n ? pl.id[i] : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, e);
-      const int before = __popc(same & ((1u << lane) - 1));
-      int base = 0;
-      if (e >= 0) base = pl.list[e];
-      __syncwarp();
-      if (e >= 0 && before == 0) pl.list[e] = static_cast<int16_t>(base + __popc(same));
-      __syncwarp();
-      if (e >= 0) pl.rank[i] = static_cast<int16_t>(base + before);
-    }
     int entries = 0, pairs = 0;
+#pragma unroll 1
     for (int e0 = 0; e0 <= experts; e0 += 32) {
       const int e = e0 + lane;
-      const int c = e <= experts ? pl.list[e] : 0, pieces = (c + kColumns - 1) / kColumns;
+      const int c = e <= experts ? __popcll(pl.who[e]) : 0, pieces = (c + kColumns - 1) / kColumns;
       int before = c | pieces << 16;  // inclusive sums of both
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -99,6 +106,7 @@ __device__ __forceinline__ void build_plan(Plan<kColumns>& pl, const MoePass& p)
       }
       const int first = pairs + (before & 0xffff) - c, at = entries + (before >> 16) - pieces;
       if (c > 0) pl.list[e] = static_cast<int16_t>(first);
+#pragma unroll 1
       for (int i = 0; i < pieces; ++i) {
         pl.expert[at + i] = static_cast<int16_t>(e);
         pl.start[at + i] = static_cast<int16_t>(first + i * kColumns);
@@ -110,8 +118,11 @@ __device__ __forceinline__ void build_plan(Plan<kColumns>& pl, const MoePass& p)
     if (lane == 0) pl.entries = entries, pl.start[entries] = static_cast<int16_t>(pairs);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads)
-    if (pl.id[i] >= 0) pl.pair[pl.list[pl.id[i]] + pl.rank[i]] = static_cast<int16_t>(i);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int e = pl.id[i];
+    if (e >= 0) pl.pair[pl.list[e] + __popcll(pl.who[e] & ((1ull << token(i)) - 1))] = static_cast<int16_t>(i);
+  }
   __syncthreads();
 }
 
@@ -163,6 +174,7 @@ struct Product {
   const MoeWeights& w;
   const P& pl;
   uint8_t *smem, *scale_smem;
+  int room;  // bytes for columns
   TileGroup g;
   bool dense;
   int per_cta, tiles, pairs, from, to, end;  // [from, to) is the segment
@@ -173,16 +185,17 @@ struct Product {
     int entry, tile;
   } first, loading, fetching, now;
 
-  __device__ __forceinline__ Product(const MoePass& p_, const MoeWeights& w_, const P& pl_, uint8_t* smem_,
+  __device__ __forceinline__ Product(const MoePass& p_, const MoeWeights& w_, const P& pl_, uint8_t* smem_, int room_,
                                      uint8_t* scale_smem_, int warps, bool dense_)
-      : p(p_), w(w_), pl(pl_), smem(smem_), scale_smem(scale_smem_), g(warps), dense(dense_) {
+      : p(p_), w(w_), pl(pl_), smem(smem_), scale_smem(scale_smem_), room(room_), g(warps), dense(dense_) {
     per_cta = kWarps / g.warps;
     tiles = kUp ? p.inner / 8 : p.hidden / 16;  // of a routed entry
     pairs = p.tokens * p.routing.top_k;
     const int shared_tiles = kUp ? p.shared_inner / 8 : tiles;
-    const int64_t items = static_cast<int64_t>(pl.routed) * tiles + static_cast<int64_t>(pl.entries - pl.routed) * shared_tiles;
-    from = to = static_cast<int>(items * blockIdx.x / gridDim.x);
-    end = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
+    // at most 1100 entries of a few thousand tiles: the products fit 32 bits
+    const uint32_t items = pl.routed * tiles + (pl.entries - pl.routed) * shared_tiles;
+    from = to = items / gridDim.x * blockIdx.x + items % gridDim.x * blockIdx.x / gridDim.x;
+    end = items / gridDim.x * (blockIdx.x + 1) + items % gridDim.x * (blockIdx.x + 1) / gridDim.x;
   }
   __device__ __forceinline__ int tiles_of(int entry) const { return kUp && entry >= pl.routed ? p.shared_inner / 8 : tiles; }
   __device__ __forceinline__ int k_of(int entry) const {
@@ -190,6 +203,7 @@ struct Product {
   }
   __device__ __forceinline__ void move(Place& at, int by) const {
     at.tile += by;
+#pragma unroll 1
     for (int n = tiles_of(at.entry); at.tile >= n && at.entry + 1 < pl.entries; n = tiles_of(at.entry)) at.tile -= n, ++at.entry;
   }
   // The matrix of a tile's rows, and the number of its fragment row r.
@@ -205,19 +219,21 @@ struct Product {
     if (!kUp) return at.tile * 16 + r;
     return at.tile * 8 + (r < 8 ? r : r - 8 + rows_of(at.entry) / 2);
   }
-  // What the ring asks of its source.
-  __device__ __forceinline__ void rows(WCursor<F>& cur, int i) {
+  // What the stream asks of its source.
+  __device__ __forceinline__ TileRows rows(int i) {
     if (i > 0) move(loading, per_cta);
     int64_t e;
     const MoeMatrix& m = matrix(loading, e);
     const int n = rows_of(loading.entry), k = k_of(loading.entry), lane = threadIdx.x & 31;
+    TileRows t;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int at = row(loading, (lane >> 2) + 8 * r);
-      cur.data[r] = m.data + (e * n + at) * W::row_bytes(k) + (lane & 3) * 16;
+      t.data[r] = m.data + (e * n + at) * W::row_bytes(k) + (lane & 3) * 16;
       if constexpr (F == kWFp8)
-        cur.scale[r] = static_cast<const float*>(m.scale) + (e * ((n + 127) / 128) + at / 128) * ((k + 127) / 128);
+        t.scale[r] = static_cast<const float*>(m.scale) + (e * ((n + 127) / 128) + at / 128) * ((k + 127) / 128);
     }
+    return t;
   }
   __device__ __forceinline__ bool zeros() const { return (kUp ? w.w13.zero : w.w2.zero) != nullptr || (kUp ? w.shared13.zero : w.shared2.zero) != nullptr; }
   __device__ __forceinline__ WScales scales_of(const Place& at, int r) const {
@@ -243,9 +259,10 @@ struct Product {
   __device__ __forceinline__ int token(int pair) const { return pair < pairs ? pair / p.routing.top_k : pair - pairs; }
 
   // Starts the loads of the next segment, the run of tiles that one layout of
-  // columns serves: all with dense columns, else those of one entry.
-  template <typename Ring>
-  __device__ __forceinline__ bool start(Ring& ring) {
+  // columns serves: with dense columns all, else those of as many entries as
+  // shared memory holds the columns of (of one reduction length).
+  template <typename Stream>
+  __device__ __forceinline__ bool start(Stream& stream) {
     from = to;
     if (from >= end) return false;
     const int routed_items = pl.routed * tiles;
@@ -256,47 +273,76 @@ struct Product {
       first_entry = (from - routed_items) / n, tile = from - routed_items - first_entry * n;
       first_entry += pl.routed;
     }
-    to = dense ? end : min(end, from - tile + tiles_of(first_entry));
+    to = end;
+    if (!dense) {
+      const int hold = max(1, room / static_cast<int>(X::bytes(W::units(k_of(first_entry)))));
+      to = min(end, from - tile + hold * tiles_of(first_entry));
+      if (first_entry < pl.routed) to = min(to, routed_items);
+    }
     first = {first_entry, tile};
     move(first, g.id);
     loading = fetching = now = first;
-    ring.start(k_of(first_entry), g, to - from > g.id ? (to - from - g.id + per_cta - 1) / per_cta : 0, scale_smem, *this);
+    stream.start(k_of(first_entry), g, to - from > g.id ? (to - from - g.id + per_cta - 1) / per_cta : 0, scale_smem, *this);
     return true;
   }
 
   // Lays out the segment's columns and consumes its tiles.  Both ends are
   // block barriers for the columns.
-  template <typename Ring>
-  __device__ __forceinline__ void run(Ring& ring, TileSums<NB>& ts) {
-    const int k = k_of(first_entry), l0 = pl.start[first_entry];
-    const int columns = dense ? p.tokens : pl.start[first_entry + 1] - l0;
-    const int live = (columns + kWidth - 1) / kWidth;
+  template <typename Stream>
+  __device__ __forceinline__ void run(Stream& stream, TileSums<NB>& ts) {
+    ts.half = 0;  // groups of other warps may have taken another number of tiles
+    const int k = k_of(first_entry);
+    const int64_t tile_bytes = X::bytes(W::units(k));
+    Place end_at = {first_entry, 0};
+    if (!dense) {
+      // the segment's last entry
+      end_at.tile = to - 1 - (first_entry < pl.routed ? first_entry * tiles : pl.routed * tiles + (first_entry - pl.routed) * tiles_of(pl.routed));
+      move(end_at, 0);
+    }
+    int most = 0;  // blocks of columns of an entry
+#pragma unroll 1
+    for (int entry = first_entry; entry <= end_at.entry; ++entry) {
+      const int l0 = pl.start[entry];
+      const int columns = dense ? p.tokens : pl.start[entry + 1] - l0;
+      most = max(most, (columns + kWidth - 1) / kWidth);
+    }
+#pragma unroll 1
+    for (int entry = first_entry; entry <= end_at.entry; ++entry) {
+      const int l0 = pl.start[entry];
+      X xt(smem + (entry - first_entry) * tile_bytes, W::units(k));
+      xt.stage(k, dense ? p.tokens : pl.start[entry + 1] - l0, most, [&](int col) -> const __nv_bfloat16* {
+        if (kUp && dense)
+          return p.routing.mask == nullptr || p.routing.mask[col] ? p.x + col * p.x_stride : nullptr;
+        const int pair = pl.pair[l0 + col];
+        return kUp ? p.x + token(pair) * p.x_stride : h_row(pair);
+      });
+    }
     X xt(smem, W::units(k));
-    xt.stage(k, columns, live, [&](int col) -> const __nv_bfloat16* {
-      if (kUp && dense)
-        return p.routing.mask == nullptr || p.routing.mask[col] ? p.x + col * p.x_stride : nullptr;
-      const int pair = pl.pair[l0 + col];
-      return kUp ? p.x + token(pair) * p.x_stride : h_row(pair);
-    });
+    auto select = [&]() {
+      if (!dense) xt = X(smem + (now.entry - first_entry) * tile_bytes, W::units(k));
+    };
+    select();
     float acc[NB][4] = {};
     auto finish = [&](int, const float* sums) {
       constexpr int kCols = kUp ? 8 : 16;
       const int s0 = pl.start[now.entry], n = (pl.start[now.entry + 1] - s0) * kCols;
+#pragma unroll 1
       for (int i = g.thread(); i < n; i += g.threads()) {
         const int pair = pl.pair[s0 + i / kCols], c = i % kCols;
         const int col = dense ? token(pair) : i / kCols;
         const float v = TileSums<NB>::sum(sums, g, c, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
         if (kUp) {
           const float up = TileSums<NB>::sum(sums, g, c + 8, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
-          h_row(pair)[now.tile * 8 + c] = __float2bfloat16_rn(v / (1.0f + expf(-v)) * up * pl.weight[pair]);
+          h_row(pair)[now.tile * 8 + c] = __float2bfloat16_rn(__fdividef(v, 1.0f + __expf(-v)) * up * pl.weight[pair]);
         } else {
           p.part[static_cast<int64_t>(pair) * p.hidden + now.tile * 16 + c] = v;
         }
       }
       move(now, per_cta);
+      select();
     };
-    if (NB > 1 && live == 1) ring.template run<1>(xt, g, ts, acc, *this, finish);
-    else ring.template run<NB>(xt, g, ts, acc, *this, finish);
+    if (NB > 1 && most == 1) stream.template run<1>(xt, g, ts, acc, *this, finish);
+    else stream.template run<NB>(xt, g, ts, acc, *this, finish);
     __syncthreads();
   }
 };
@@ -308,28 +354,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Plan<NB * kWidth> pl;
   extern __shared__ __align__(16) uint8_t smem[];
   build_plan(pl, p);
-  TileRing<F, __nv_bfloat16> ring;
-  uint8_t* sums = smem + X::bytes(WTraits<F>::units(max(p.hidden, max(p.inner, p.shared_inner))));
+  TileStream<F, __nv_bfloat16> stream;
+  const int room = static_cast<int>(X::bytes(WTraits<F>::units(max(p.hidden, max(p.inner, p.shared_inner)))));
+  uint8_t* sums = smem + room;
   TileSums<NB> ts(sums);
   uint8_t* scales = sums + TileSums<NB>::bytes(kWarps);
   {
-    Product<F, NB, kWidth, true> up(p, w, pl, smem, scales, shape.up_warps, shape.dense);
-    while (up.start(ring)) up.run(ring, ts);
+    Product<F, NB, kWidth, true> up(p, w, pl, smem, room, scales, shape.up_warps, shape.dense);
+    while (up.start(stream)) up.run(stream, ts);
   }
   grid_arrive(p.barrier);
   {
-    Product<F, NB, kWidth, false> down(p, w, pl, smem, scales, shape.down_warps, false);
-    bool more = down.start(ring);
+    Product<F, NB, kWidth, false> down(p, w, pl, smem, room, scales, shape.down_warps, false);
+    bool more = down.start(stream);
     if (!grid_wait(p.barrier, 1, p.error)) return;
     while (more) {
-      down.run(ring, ts);
-      more = down.start(ring);
+      down.run(stream, ts);
+      more = down.start(stream);
     }
   }
   grid_arrive(p.barrier);
   if (!grid_wait(p.barrier, 2, p.error)) return;
   // y: a token's shares, in the order of its slots, four columns a thread
   const int quads = p.hidden / 4, top_k = p.routing.top_k;
+#pragma unroll 1
   for (int i = blockIdx.x * kThreads + threadIdx.x; i < p.tokens * quads; i += gridDim.x * kThreads) {
     const int t = i / quads, n = (i - t * quads) * 4;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -358,14 +406,13 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr || w.shared13.zero != nullptr || w.shared2.zero != nullptr;
   auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
   // Warps to a tile: as few as leave every group of every SM two tiles (if
-  // every pair chose another expert) and room for the scales, but at least four
-  // units a warp (one step of its ring), or one where the tiles are too few to
-  // fill the machine otherwise.
+  // every pair chose another expert) and room for the scales, but at least one
+  // quad of units a warp.
   auto warps = [&](int64_t tiles, int64_t shared_tiles, int k, int least_k) {
     const int64_t n = std::min(p.routing.experts, p.tokens * p.routing.top_k) * tiles + shared_tiles;
     int gw = 1;
-    while (gw < kWarps && 2 * gw <= W::units(least_k) &&
-           (n < (W::units(least_k) >= 8 * gw ? 2ll : 1ll) * sms * (kWarps / gw) || columns + scales(k, gw) > kSmem))
+    while (gw < kWarps && 8 * gw <= W::units(least_k) &&
+           (n < 2ll * sms * (kWarps / gw) || columns + scales(k, gw) > kSmem))
       gw *= 2;
     return gw;
   };

@@ -16,12 +16,12 @@
 // A "unit" is the piece of a row that the four lanes of a fragment row hold
 // at a time, 16 bytes a lane in one load: 32 bf16, 64 e4m3 or 128 4-bit codes.
 // (A load costs L1 a cycle for each of its eight rows whatever its width, so
-// narrower ones would cap the rate.)  A warp keeps four units on their way in
-// registers, across the ends of tiles.  Rings in shared memory, filled by TMA
-// boxes or asynchronous copies, were slower (3.7 TB/s where this came to 4.8):
-// each unit then starts with a wait and a read that nothing overlaps.  So were
-// loops that keep one copy of the code for tiles' ends: where paths meet the
-// compiler has to wait for every load under way.  A product may only sum
+// narrower ones would cap the rate.)  A warp works in quads of units, the next
+// quad on its way in registers while one is consumed, across the ends of
+// tiles; rows are padded to whole quads with activations that are zero, so the
+// loop over quads has no branches.  (Rings in shared memory, filled by TMA
+// boxes or asynchronous copies, came to 3.7 TB/s where this comes to 5: each
+// unit then starts with a wait and a read that nothing overlaps.)  A product may only sum
 // over one group of codes; with groups of 64 or 32 the four lanes exchange
 // words first.  Sums are held in 32 bits; group and block scales multiply the
 // 32-bit sums of their own groups.  The 4-bit scales and zero points of a
@@ -62,12 +62,11 @@ struct WTraits {
   static constexpr int kSub = F == kW4G32 ? 4 : F == kW4G64 ? 2 : 1;  // groups of a unit
   static constexpr int kPieces = kUnitK / 32;    // 16-byte activation pieces of a lane and column
   static constexpr int kGroupK = kUnitK / kSub;  // reduction length of a group
-  // k may end inside a unit
-  static constexpr bool kRagged = F == kWFp8 || F == kW4G32 || F == kW4G64;
   __host__ __device__ static constexpr int64_t row_bytes(int64_t k) {
     return F == kWBf16 ? 2 * k : F == kWFp8 ? k : k / 2;
   }
-  __host__ __device__ static constexpr int units(int k) { return (k + kUnitK - 1) / kUnitK; }
+  // units of rows of k, in whole quads
+  __host__ __device__ static constexpr int units(int k) { return (k + 4 * kUnitK - 1) / (4 * kUnitK) * 4; }
 };
 
 template <typename T>
@@ -190,14 +189,14 @@ __device__ __forceinline__ uint4 piece_order(uint4 v) {
 }
 
 // The warps that share a tile: warp `index` of `warps`, group `id` of the
-// block.  They take the tile's units in even runs and add their sums here.
+// block.  They take the tile's quads of units in even runs.
 struct TileGroup {
   int warps, index, id;
 
   __device__ __forceinline__ explicit TileGroup(int warps_)
       : warps(warps_), index((threadIdx.x >> 5) % warps_), id((threadIdx.x >> 5) / warps_) {}
-  __device__ __forceinline__ int first_unit(int units) const { return units * index / warps; }
-  __device__ __forceinline__ int end_unit(int units) const { return units * (index + 1) / warps; }
+  __device__ __forceinline__ int first_unit(int units) const { return units / 4 * index / warps * 4; }
+  __device__ __forceinline__ int end_unit(int units) const { return units / 4 * (index + 1) / warps * 4; }
   __device__ __forceinline__ int threads() const { return warps * 32; }
   __device__ __forceinline__ int thread() const { return index * 32 + (threadIdx.x & 31); }
 
@@ -228,12 +227,12 @@ struct ScaleTile {
 
   // bytes of a row: n scales and n zero points, each with room for words'
   // edges; an odd number of 16 bytes, so that eight rows start in different banks
-  __host__ __device__ static int zero_offset(int n) { return (2 * n + 15) / 16 * 16 + (n % 8 ? 16 : 0); }
+  __host__ __device__ static int zero_offset(int n) { return (2 * n + 4 + 15) / 16 * 16; }
   __host__ __device__ static int row_pitch(int n, bool zeros) {
     return ((zero_offset(n) + (zeros ? n + 8 : 0) + 15) / 16 | 1) * 16;
   }
   // most groups of a warp's share
-  __host__ __device__ static int share(int units, int warps) { return (units + warps - 1) / warps * W::kSub; }
+  __host__ __device__ static int share(int units, int warps) { return (units / 4 + warps - 1) / warps * 4 * W::kSub; }
   __host__ __device__ static int64_t bytes(int units, bool zeros, int group_warps, int block_warps) {
     return W::kIs4 ? 32ll * block_warps * row_pitch(share(units, group_warps), zeros) : 0;
   }
@@ -251,6 +250,7 @@ struct ScaleTile {
     const int lane = threadIdx.x & 31, half = lane >> 4;
     const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(row(i, lane & 15)));
     if (wide) {
+#pragma unroll 1
       for (int g = g0 + 8 * half; g < g1; g += 16) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 2 * (g - g0)), "l"(from.scale + 2 * g) : "memory");
         if (from.zero != nullptr)
@@ -264,6 +264,7 @@ struct ScaleTile {
   static __device__ __forceinline__ void copy(uint32_t to, const uint8_t* from, const uint8_t* until, const uint8_t* end, int first) {
     const uint8_t* p = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t{3}) + 4 * first;
     to += 4 * first;
+#pragma unroll 1
     for (; p < until; p += 8, to += 8) {
       const int n = static_cast<int>(min(static_cast<int64_t>(4), static_cast<int64_t>(end - p)));  // not past the array
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to), "l"(p), "r"(n) : "memory");
@@ -299,11 +300,13 @@ struct XTile {
     const int padded = units * W::kUnitK;
     // several columns' loads under way at a time
     constexpr int kAhead = kWidth;
+#pragma unroll 1
     for (int c0 = 0; c0 < live * kWidth; c0 += kAhead) {
       const T* p[kAhead];
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) p[n] = c0 + n < columns ? row(c0 + n) : nullptr;
       uint4* to = pieces + c0 / kWidth * units * kUnitPieces;
+#pragma unroll 1
       for (int i = threadIdx.x * 8; i < padded; i += blockDim.x * 8) {
         uint4 v[kAhead];
 #pragma unroll
@@ -318,6 +321,7 @@ struct XTile {
     if constexpr (W::kIs4) {
       const int lane = threadIdx.x & 31;
       const int groups = live * units * W::kSub;
+#pragma unroll 1
       for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
         constexpr int kEach = W::kPieces / W::kSub;
         float v = 0.0f;
@@ -461,48 +465,45 @@ __device__ __forceinline__ void load_weights(uint32_t (&w)[4], const uint8_t* p)
                : "l"(p));
 }
 
-// The lane's two rows of a tile (fragment rows lane / 4 and lane / 4 + 8) and
-// the unit of them to load next.  data[] starts 16 (lane % 4) bytes into the row.
-template <int F>
-struct WCursor {
+// The lane's two rows of a tile (fragment rows lane / 4 and lane / 4 + 8), from
+// 16 (lane % 4) bytes on.
+struct TileRows {
   const uint8_t* data[2];
   const float* scale[2];  // e4m3: of the row's blocks
-  int unit;
 };
 
-// Units of a run of tiles on their way, kDepth of them, across the ends of
-// tiles.  `source` knows the tiles: source.rows(cur, i) points the cursor at
-// the rows of the group's i-th tile, source.scales(i, row) tells where the
-// scales of a row of it are and source.here the same for the tile now consumed,
-// source.zeros whether there are zero points (4-bit only).  Each is asked for
-// the tiles in order.
+// A warp's share of a run of tiles.  `source` knows the tiles: source.rows(i)
+// are the lane's rows of the group's i-th tile, source.scales(i, row) tells
+// where the scales of a row of it are and source.here the same for the tile now
+// consumed, source.zeros whether there are zero points (4-bit only).  Each is
+// asked for the tiles in order.  finish(i, sums) may move xt to the next tile's
+// columns.
 template <int F, typename T>
-struct TileRing {
+struct TileStream {
   using W = WTraits<F>;
-  static constexpr int kDepth = 4;
-  struct Step {
+  struct Unit {
     uint32_t w[2][4];
     float s[2];  // e4m3
-  } st[kDepth];
-  WCursor<F> cur;
+  } quad[4];
+  TileRows at;  // of the tile whose first quad is on its way
   ScaleTile<F> sc;
-  int k, u0, u1, next, count, g0, g1;
+  int k, u0, u1, count, g0, g1;
 
-  // Lanes whose share of a row's last unit lies past its end read its last
-  // bytes again; the activations there are zeros.
-  template <typename Source>
-  __device__ __forceinline__ void load(Step& s, Source& source) {
-    if (next >= count) return;
-    int off = cur.unit * 64;
-    if (W::kRagged) off = min(off, static_cast<int>(W::row_bytes(k)) - 16 * (1 + (static_cast<int>(threadIdx.x) & 3)));
+  // Units u .. u + 3.  What lies past the end of a row reads as its last bytes
+  // again; the activations there are zeros.
+  template <bool kWhole>
+  __device__ __forceinline__ void load(const TileRows& from, int u) {
+    const int last = static_cast<int>(W::row_bytes(k)) - 16 * (1 + (static_cast<int>(threadIdx.x) & 3));
+#pragma unroll
+    for (int d = 0; d < 4; ++d) load_unit<kWhole>(quad[d], from, u, d, last);
+  }
+  template <bool kWhole>
+  __device__ __forceinline__ void load_unit(Unit& to, const TileRows& from, int u, int d, int last) const {
+    const int off = kWhole ? u * 64 : min((u + d) * 64, last);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      load_weights(s.w[r], cur.data[r] + off);
-      if (F == kWFp8) s.s[r] = __ldg(cur.scale[r] + cur.unit / 2);  // blocks of 128
-    }
-    if (++cur.unit == u1) {
-      cur.unit = u0;
-      if (++next < count) source.rows(cur, next);
+      load_weights(to.w[r], from.data[r] + off + (kWhole ? d * 64 : 0));
+      if (F == kWFp8) to.s[r] = __ldg(from.scale[r] + (kWhole ? (u + d) / 2 : min((u + d) / 2, (k - 1) / 128)));  // blocks of 128
     }
   }
   template <typename Source>
@@ -517,13 +518,13 @@ struct TileRing {
   template <typename Source>
   __device__ __forceinline__ void start(int k_, const TileGroup& g, int count_, uint8_t* smem, Source& source) {
     const int units = W::units(k_);
-    k = k_, u0 = g.first_unit(units), u1 = g.end_unit(units), next = 0, count = count_;
-    cur.unit = u0;
-    if (count > 0) source.rows(cur, 0);
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) load(st[d], source);
+    k = k_, u0 = g.first_unit(units), u1 = g.end_unit(units), count = count_;
+    if (count > 0) {
+      at = source.rows(0);
+      load<false>(at, u0);
+    }
     if constexpr (W::kIs4) {
-      g0 = u0 * W::kSub, g1 = min(u1 * W::kSub, k / W::kGroupK);
+      g0 = min(u0 * W::kSub, k / W::kGroupK), g1 = min(u1 * W::kSub, k / W::kGroupK);
       sc.init(smem, units, source.zeros(), g.warps, k / W::kGroupK, g0, g1);
       __syncwarp();  // the last run's scales have been read
       fetch_scales(0, source);
@@ -532,10 +533,17 @@ struct TileRing {
   }
   // Consumes them; finish(i, sums) for each tile, in order.
   template <int NBL, typename X, typename Sums, int NB, typename Source, typename Finish>
-  __device__ __forceinline__ void run(const X& xt, const TileGroup& g, Sums& ts, float (&acc)[NB][4], Source& source, Finish finish) {
-    int u = u0, i = 0;
-    const uint8_t *srow[2], *zrow[2];  // of the lane's rows, at group 0
-    auto begin_tile = [&]() {
+  __device__ __forceinline__ void run(X& xt, const TileGroup& g, Sums& ts, float (&acc)[NB][4], Source& source, Finish finish) {
+    if (k % (4 * W::kUnitK) == 0) run_tiles<NBL, true>(xt, g, ts, acc, source, finish);
+    else run_tiles<NBL, false>(xt, g, ts, acc, source, finish);
+  }
+  template <int NBL, bool kWhole, typename X, typename Sums, int NB, typename Source, typename Finish>
+  __device__ __forceinline__ void run_tiles(X& xt, const TileGroup& g, Sums& ts, float (&acc)[NB][4], Source& source, Finish finish) {
+    const bool zeros = W::kIs4 && source.zeros();
+    const int last = static_cast<int>(W::row_bytes(k)) - 16 * (1 + (static_cast<int>(threadIdx.x) & 3));
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      const uint8_t *srow[2], *zrow[2];  // of the lane's rows, at group 0
       if constexpr (W::kIs4) {
         asm volatile("cp.async.wait_group 1;\n" ::: "memory");  // all but the next tile's
         __syncwarp();
@@ -551,37 +559,43 @@ struct TileRing {
           }
         }
       }
-    };
-    const bool zeros = W::kIs4 && source.zeros();
-    auto scales = [&](int d, int j, float (&s)[2], float (&z)[2]) {
-      if constexpr (W::kIs4) {
-        const int n = u * W::kSub + j;
-        const bool in = !W::kRagged || n < g1;  // no group: x is zero there
+      const TileRows here = at;
+      if (i + 1 < count) at = source.rows(i + 1);
+#pragma unroll 1
+      for (int u = u0; u < u1; u += 4) {
+        // the quad after this one: the tile's next, or the next tile's first
+        // (after the last tile its own first again, which nothing reads)
+        const bool ends = u + 4 >= u1;
+        TileRows from;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          s[r] = in ? MmaType<T>::to_float(*reinterpret_cast<const uint16_t*>(srow[r] + 2 * n)) : 0.0f;
-          z[r] = zeros ? static_cast<float>(zrow[r][n]) : 8.0f;
+          from.data[r] = ends ? at.data[r] : here.data[r];
+          if (F == kWFp8) from.scale[r] = ends ? at.scale[r] : here.scale[r];
         }
-      } else {
-        s[0] = st[d].s[0], s[1] = st[d].s[1];
-      }
-    };
-    if (count > 0) begin_tile();
-    while (i < count) {
+        const int next = ends ? u0 : u + 4;
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        xt.template consume<NBL>(acc, st[d].w, u, [&](int j, float (&s)[2], float (&z)[2]) { scales(d, j, s, z); });
-        load(st[d], source);
-        if (++u < u1) continue;
-        if constexpr (W::kIs4) {
-          __syncwarp();  // this tile's scales have been read
-          fetch_scales(i + 2, source);
+        for (int d = 0; d < 4; ++d) {
+          xt.template consume<NBL>(acc, quad[d].w, u + d, [&](int j, float (&s)[2], float (&z)[2]) {
+            if constexpr (W::kIs4) {
+              const int n = (u + d) * W::kSub + j;
+              const bool in = kWhole || n < g1;  // no group: x is zero there
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                s[r] = in ? MmaType<T>::to_float(*reinterpret_cast<const uint16_t*>(srow[r] + 2 * n)) : 0.0f;
+                z[r] = zeros ? static_cast<float>(zrow[r][n]) : 8.0f;
+              }
+            } else {
+              s[0] = quad[d].s[0], s[1] = quad[d].s[1];
+            }
+          });
+          load_unit<kWhole>(quad[d], from, next, d, last);
         }
-        finish(i, ts.join(acc, g));
-        u = u0;
-        if (++i >= count) break;
-        begin_tile();
       }
+      if constexpr (W::kIs4) {
+        __syncwarp();  // this tile's scales have been read
+        fetch_scales(i + 2, source);
+      }
+      finish(i, ts.join(acc, g));
     }
   }
 };

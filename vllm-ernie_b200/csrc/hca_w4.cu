@@ -6,7 +6,7 @@
 // x in shared memory and walks over tiles of 16 rows of W.  The warps form
 // groups; a group's warps split the reduction of its tile and their 32-bit
 // sums meet in shared memory in warp order, so results do not depend on
-// timing.  Each warp keeps kDepth units in flight, across the ends of tiles.
+// timing.
 #include "hca_stream.cuh"
 
 #include <algorithm>
@@ -40,10 +40,12 @@ struct W4Tiles {
   __device__ __forceinline__ int64_t row(int i, int r) const {
     return min((first + i * stride) * 16 + r, a.n - 1);  // rows past the end are read again, not stored
   }
-  __device__ __forceinline__ void rows(WCursor<F>& cur, int i) const {
+  __device__ __forceinline__ TileRows rows(int i) const {
     const int lane = threadIdx.x & 31;
+    TileRows t;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) cur.data[r] = a.q + (lane & 3) * 16 + row(i, (lane >> 2) + 8 * r) * W::row_bytes(a.k);
+    for (int r = 0; r < 2; ++r) t.data[r] = a.q + (lane & 3) * 16 + row(i, (lane >> 2) + 8 * r) * W::row_bytes(a.k);
+    return t;
   }
   __device__ __forceinline__ bool zeros() const { return a.zeros != nullptr; }
   __device__ __forceinline__ WScales here(int i, int r) const {
@@ -69,8 +71,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   W4Tiles<F, T> src{a, static_cast<int>(blockIdx.x) * per_cta + g.id, static_cast<int>(gridDim.x) * per_cta, a.k / W::kGroupK};
 
   pdl_wait_and_release();
-  TileRing<F, T> ring;
-  ring.start(a.k, g, src.first < tiles ? (tiles - src.first + src.stride - 1) / src.stride : 0,
+  TileStream<F, T> stream;
+  stream.start(a.k, g, src.first < tiles ? (tiles - src.first + src.stride - 1) / src.stride : 0,
              smem + X::bytes(units) + TileSums<NB>::bytes(kWarps), src);
   const T* x = static_cast<const T*>(a.x) + t0 * a.x_stride;
   xt.stage(a.k, columns, live, [&](int col) { return x + col * a.x_stride; });
@@ -78,6 +80,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   float acc[NB][4] = {};
   auto finish = [&](int i, const float* sums) {
     const int row0 = (src.first + i * src.stride) * 16;
+#pragma unroll 1
     for (int j = g.thread(); j < live * 128; j += g.threads()) {
       const int row = row0 + (j & 15), block = j >> 7, col = (j >> 4) & 7, t = block * kWidth + col;
       if (row < a.n && col < kWidth && t < columns)
@@ -85,8 +88,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
             MmaType<T>::from_float(TileSums<NB>::sum(sums, g, j & 15, block, col) * Scaling<F, T>::kOut);
     }
   };
-  if (NB > 1 && live == 1) ring.template run<1>(xt, g, ts, acc, src, finish);
-  else ring.template run<NB>(xt, g, ts, acc, src, finish);
+  if (NB > 1 && live == 1) stream.template run<1>(xt, g, ts, acc, src, finish);
+  else stream.template run<NB>(xt, g, ts, acc, src, finish);
 }
 
 // Launches with NB blocks of kWidth columns if shared memory holds them.
@@ -96,13 +99,11 @@ bool launch(W4Args a, cudaStream_t s, int& rc) {
   const int64_t columns = XTile<F, T, NB, kWidth>::bytes(units) + TileSums<NB>::bytes(kWarps);
   auto scales = [&](int warps) { return ScaleTile<F>::bytes(units, a.zeros != nullptr, warps, kWarps); };
   // Warps to a tile: as few as leave every SM's groups four tiles each and
-  // room for the scales, but at least four units a warp (one step of its
-  // ring), or one where the tiles are too few to fill the machine otherwise.
-  // Few warps mean long runs between reductions.
+  // room for the scales, but at least one quad a warp.  Few warps mean long
+  // runs between reductions, many that a short matrix still fills the machine.
   a.group_warps = 1;
-  while (a.group_warps < kWarps && 2 * a.group_warps <= units &&
-         (tiles < (units >= 8 * a.group_warps ? 4ll : 1ll) * sms * (kWarps / a.group_warps) ||
-          columns + scales(a.group_warps) > kSmem))
+  while (a.group_warps < kWarps && 8 * a.group_warps <= units &&
+         (tiles < 4ll * sms * (kWarps / a.group_warps) || columns + scales(a.group_warps) > kSmem))
     a.group_warps *= 2;
   const int64_t smem = columns + scales(a.group_warps);
   if (smem > kSmem) return false;
