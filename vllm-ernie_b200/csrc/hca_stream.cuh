@@ -485,7 +485,7 @@ struct TileStream {
     uint32_t w[2][4];
     float s[2];  // e4m3
   } quad[4];
-  TileRows at;  // of the tile whose first quad is on its way
+  TileRows at;  // of the tile whose units are loaded next
   ScaleTile<F> sc;
   int k, u0, u1, count, g0, g1;
 
@@ -559,19 +559,12 @@ struct TileStream {
           }
         }
       }
-      const TileRows here = at;
-      if (i + 1 < count) at = source.rows(i + 1);
 #pragma unroll 1
       for (int u = u0; u < u1; u += 4) {
         // the quad after this one: the tile's next, or the next tile's first
         // (after the last tile its own first again, which nothing reads)
         const bool ends = u + 4 >= u1;
-        TileRows from;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          from.data[r] = ends ? at.data[r] : here.data[r];
-          if (F == kWFp8) from.scale[r] = ends ? at.scale[r] : here.scale[r];
-        }
+        if (ends && i + 1 < count) at = source.rows(i + 1);
         const int next = ends ? u0 : u + 4;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
@@ -588,7 +581,7 @@ struct TileStream {
               s[0] = quad[d].s[0], s[1] = quad[d].s[1];
             }
           });
-          load_unit<kWhole>(quad[d], from, next, d, last);
+          load_unit<kWhole>(quad[d], at, next, d, last);
         }
       }
       if constexpr (W::kIs4) {
