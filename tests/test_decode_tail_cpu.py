@@ -59,7 +59,7 @@ def test_moe_workspace_is_for_one_pass_and_the_routing():
     assert f(0, 64, 8, 4096, 1024, 0) == 0 and f(1, 64, 8, 4096, 0, 0) == 0
     assert f(1, 64, 8, 4096, 1024, 0) >= 8 * 1024 * 2 + 9 * 4096 * 4 + 64 * 4
     # the intermediates of 64 tokens at most, however many tokens follow
-    assert f(1000, 64, 8, 4096, 1024, 512) < f(64, 64, 8, 4096, 1024, 512) + 1000 * 64 * 4 + 1024
+    assert f(1000, 64, 8, 4096, 1024, 512) < f(64, 64, 8, 4096, 1024, 512) + 1000 * (64 + 2 * 8) * 4 + 1024
 
 
 def test_route_statuses():

@@ -133,6 +133,11 @@ __global__ void __launch_bounds__(kWarps * 32)
   });
 }
 
+int choose(int32_t* ids, float* weights, const float* logits, int tokens, const MoeRouting& r, cudaStream_t s) {
+  return launch_pdl(moe_choose_kernel, dim3(cdiv(tokens, kWarps)), dim3(kWarps * 32), 0, s, ids, weights, logits, tokens,
+                    r);
+}
+
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 int check_sizes(int tokens, int experts, int hidden, int top_k) {
@@ -162,7 +167,7 @@ int64_t logit_bytes(int tokens, int experts) { return align_up(static_cast<int64
 // Scratch of a call: gated products and the pairs' shares of y of one pass,
 // a barrier word a pass, and the logits.
 struct Scratch {
-  int64_t h, part, barriers, logits, total;
+  int64_t h, part, barriers, logits, ids, weights, total;
   int passes;
   Scratch(int tokens, int experts, int top_k, int hidden, int inner, int shared_inner) {
     const int64_t t = std::min(tokens, kMoeTokens);
@@ -171,7 +176,9 @@ struct Scratch {
     part = align_up(t * (static_cast<int64_t>(top_k) * inner + shared_inner) * 2);
     barriers = part + align_up(t * (top_k + 1) * hidden * 4);
     logits = barriers + align_up(4ll * passes);
-    total = logits + logit_bytes(tokens, experts);
+    ids = logits + logit_bytes(tokens, experts);
+    weights = ids + align_up(4ll * tokens * top_k);
+    total = weights + align_up(4ll * tokens * top_k);
   }
 };
 
@@ -261,8 +268,7 @@ extern "C" int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_
   rc = compute_logits(logits, x, x_stride, router, router_fp32, num_tokens, num_experts, hidden, nullptr, 0, s);
   if (rc != HCA_OK) return rc;
   const MoeRouting r{router_bias, token_mask, num_experts, top_k, sigmoid, renormalize, routed_scale};
-  return launch_pdl(moe_choose_kernel, dim3(cdiv(num_tokens, kWarps)), dim3(kWarps * 32), 0, s, ids, weights, logits,
-                    num_tokens, r);
+  return choose(ids, weights, logits, num_tokens, r, s);
 }
 
 extern "C" int64_t hca_moe_workspace_bytes(int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,
@@ -330,6 +336,17 @@ extern "C" int hca_moe_decode(void* out, int64_t out_stride, const void* x, int6
                       reinterpret_cast<uint32_t*>(scratch + at.barriers), at.passes, s);
   if (rc != HCA_OK) return rc;
   const MoeRouting r{router_bias, token_mask, num_experts, top_k, sigmoid, renormalize, routed_scale};
+  // Choosing is a warp's work a token: every CTA of the expert kernel does it
+  // while its warps do not have to take turns (2 us), else a launch does (with
+  // 64 tokens 3 us for 9).
+  if (num_tokens > 16) {
+    int32_t* ids = reinterpret_cast<int32_t*>(scratch + at.ids);
+    float* weights = reinterpret_cast<float*>(scratch + at.weights);
+    rc = choose(ids, weights, logits, num_tokens, r, s);
+    return rc != HCA_OK ? rc
+                        : experts_passes(out, out_stride, x, x_stride, nullptr, ids, weights, r, format, group_size, w,
+                                         num_tokens, hidden, inner, shared_inner, scratch, at, s);
+  }
   return experts_passes(out, out_stride, x, x_stride, logits, nullptr, nullptr, r, format, group_size, w, num_tokens,
                         hidden, inner, shared_inner, scratch, at, s);
 }

@@ -55,7 +55,7 @@ __device__ __forceinline__ void build_plan(Plan<kColumns>& pl, const MoePass& p)
   const int routed = p.tokens * top_k, n = routed + p.tokens;
   const uint8_t* mask = p.routing.mask;
 #pragma unroll 1
-  for (int e = threadIdx.x; e <= experts; e += kThreads) pl.who[e] = 0;
+  for (int e = threadIdx.x; e < experts; e += kThreads) pl.who[e] = 0;
   if (p.logits != nullptr) {
     choose_all(p.logits, p.routing, threadIdx.x >> 5, kWarps, p.tokens, [&](int t, int id, float weight) {
       pl.id[t * top_k + lane] = static_cast<int16_t>(id);
@@ -80,16 +80,20 @@ __device__ __forceinline__ void build_plan(Plan<kColumns>& pl, const MoePass& p)
       pl.weight[i] = weight;
     }
   }
-#pragma unroll 1
-  for (int t = threadIdx.x; t < p.tokens; t += kThreads) {
-    const bool in = p.shared_inner > 0 && (mask == nullptr || mask[t]);
-    pl.id[routed + t] = static_cast<int16_t>(in ? experts : -1);
-    pl.weight[routed + t] = 1.0f;
+  if (threadIdx.x < kMoeTokens) {
+    const int t = threadIdx.x;
+    const bool in = t < p.tokens && p.shared_inner > 0 && (mask == nullptr || mask[t]);
+    const uint32_t half = __ballot_sync(0xffffffffu, in);
+    if (lane == 0) reinterpret_cast<uint32_t*>(&pl.who[experts])[t / 32] = half;
+    if (t < p.tokens) {
+      pl.id[routed + t] = static_cast<int16_t>(in ? experts : -1);
+      pl.weight[routed + t] = 1.0f;
+    }
   }
   __syncthreads();
   auto token = [&](int i) { return i < routed ? i / top_k : i - routed; };
 #pragma unroll 1
-  for (int i = threadIdx.x; i < n; i += kThreads)
+  for (int i = threadIdx.x; i < routed; i += kThreads)
     if (pl.id[i] >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&pl.who[pl.id[i]]), 1ull << token(i));
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -192,10 +196,17 @@ struct Product {
     tiles = kUp ? p.inner / 8 : p.hidden / 16;  // of a routed entry
     pairs = p.tokens * p.routing.top_k;
     const int shared_tiles = kUp ? p.shared_inner / 8 : tiles;
-    // at most 1100 entries of a few thousand tiles: the products fit 32 bits
-    const uint32_t items = pl.routed * tiles + (pl.entries - pl.routed) * shared_tiles;
-    from = to = items / gridDim.x * blockIdx.x + items % gridDim.x * blockIdx.x / gridDim.x;
-    end = items / gridDim.x * (blockIdx.x + 1) + items % gridDim.x * (blockIdx.x + 1) / gridDim.x;
+    // Even shares of the units to read: a tile costs its reduction length.  (At
+    // most 1100 entries of a few thousand tiles of a few hundred units.)
+    const uint32_t cost = W::units(kUp ? p.hidden : p.inner), shared_cost = kUp || p.shared_inner == 0 ? cost : W::units(p.shared_inner);
+    const uint32_t routed_items = pl.routed * tiles, routed_cost = routed_items * cost;
+    const uint32_t all = routed_cost + (pl.entries - pl.routed) * shared_tiles * shared_cost;
+    auto boundary = [&](uint32_t block) -> int {
+      const uint32_t at = all / gridDim.x * block + all % gridDim.x * block / gridDim.x;
+      return at < routed_cost ? at / cost : routed_items + (at - routed_cost) / shared_cost;
+    };
+    from = to = boundary(blockIdx.x);
+    end = boundary(blockIdx.x + 1);
   }
   __device__ __forceinline__ int tiles_of(int entry) const { return kUp && entry >= pl.routed ? p.shared_inner / 8 : tiles; }
   __device__ __forceinline__ int k_of(int entry) const {
