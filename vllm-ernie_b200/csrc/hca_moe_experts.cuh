@@ -416,16 +416,18 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
                           TileSums<NB>::bytes(kWarps);
   const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr || w.shared13.zero != nullptr || w.shared2.zero != nullptr;
   auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
-  // Warps to a tile: as few as leave every group of every SM two tiles (if
-  // every pair chose another expert) and room for the scales, but at least one
-  // quad of units a warp.
+  // Warps to a tile: the number that makes the longest warp's work shortest (if
+  // every pair chose another expert), a tile's end costing about what a quad of
+  // units does.
   auto warps = [&](int64_t tiles, int64_t shared_tiles, int k, int least_k) {
     const int64_t n = std::min(p.routing.experts, p.tokens * p.routing.top_k) * tiles + shared_tiles;
-    int gw = 1;
-    while (gw < kWarps && 8 * gw <= W::units(least_k) &&
-           (n < 2ll * sms * (kWarps / gw) || columns + scales(k, gw) > kSmem))
-      gw *= 2;
-    return gw;
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int gw = 1; gw <= kWarps && 4 * gw <= W::units(least_k); gw *= 2) {
+      const int64_t cost = cdiv(cdiv(n, sms), kWarps / gw) * static_cast<int64_t>(cdiv(W::units(k), 4 * gw) + 1);
+      if (cost < least && columns + scales(k, gw) <= kSmem) least = cost, best = gw;
+    }
+    return best;
   };
   Shape shape;
   shape.up_warps = warps(p.inner / 8, p.shared_inner / 8, p.hidden, p.hidden);
@@ -433,8 +435,8 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
                            p.shared_inner > 0 ? std::min(p.inner, p.shared_inner) : p.inner);
   // columns that hold every token serve every expert as they are
   shape.dense = p.tokens <= NB * kWidth;
+  if (shape.up_warps == 0 || shape.down_warps == 0) return false;
   const int64_t smem = columns + std::max(scales(p.hidden, shape.up_warps), scales(inner, shape.down_warps));
-  if (smem > kSmem) return false;
   static bool done[kMaxDevices] = {};
   rc = set_func_attr_once(moe_layer_kernel<F, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
   if (rc != HCA_OK) return true;

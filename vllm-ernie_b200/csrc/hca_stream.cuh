@@ -32,8 +32,8 @@
 // spaced: bits 0..7 of a bf16 (0..10 of an fp16) with nothing above them are
 // the number times 2^-133 (2^-24), across the end of the subnormals.  So a
 // word of 4-bit codes, masked, is two codes as exact floats, and those four
-// bits higher are 16 times theirs: five bit operations for eight codes, and
-// the sums of the two kinds meet as a + b / 16.  e4m3 moved into the low
+// bits higher are 16 times theirs: five bit operations for eight codes.  e4m3
+// moved into the low
 // exponent and high mantissa bits of a bf16 is its value times 2^-120, the
 // subnormals with it.  bf16 activations are scaled by 2^80 when they are laid
 // out, so that the products keep clear of both ends of the 32-bit range for
@@ -118,6 +118,9 @@ struct Scaling {
   static constexpr bool kHalf = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
   static_assert(!kHalf || WTraits<F>::kIs4, "fp16 goes with 4-bit weights only");
   static constexpr float kX = F == kWBf16 || kHalf ? 1.0f : 0x1p80f;
+  static constexpr float kXOdd = WTraits<F>::kIs4 ? kX / 16 : kX;
+  // fp16 activations have no room for that: sums of the odd codes are held apart
+  static constexpr bool kApart = kHalf;
   static constexpr float kSum = kHalf ? 0x1p-24f : 0x1p-53f;
   static constexpr float kOut = F == kWBf16 ? 1.0f : kHalf ? 0x1p24f : F == kWFp8 ? 0x1p40f : 0x1p53f;
 };
@@ -174,17 +177,19 @@ __device__ __forceinline__ int piece_index(int k, int col) {
 
 // Eight consecutive activations in a piece's order, that in which weights come
 // out of a word together: codes 0,4 2,6 1,5 3,7 and e4m3 0,2 1,3 of each four.
+// The odd codes come out 16 times as large, which bf16 activations make up for.
 template <int F, typename T>
 __device__ __forceinline__ uint4 piece_order(uint4 v) {
   using M = MmaType<T>;
-  constexpr float kX = Scaling<F, T>::kX;
-  if constexpr (kX != 1.0f) v = make_uint4(M::times(v.x, kX), M::times(v.y, kX), M::times(v.z, kX), M::times(v.w, kX));
+  using S = Scaling<F, T>;
   if constexpr (WTraits<F>::kIs4)
-    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                      __byte_perm(v.y, v.w, 0x7632));
+    v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                   __byte_perm(v.y, v.w, 0x7632));
   if constexpr (F == kWFp8)
-    return make_uint4(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632), __byte_perm(v.z, v.w, 0x5410),
-                      __byte_perm(v.z, v.w, 0x7632));
+    v = make_uint4(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632), __byte_perm(v.z, v.w, 0x5410),
+                   __byte_perm(v.z, v.w, 0x7632));
+  if constexpr (S::kX != 1.0f)
+    v = make_uint4(M::times(v.x, S::kX), M::times(v.y, S::kX), M::times(v.z, S::kXOdd), M::times(v.w, S::kXOdd));
   return v;
 }
 
@@ -313,35 +318,21 @@ struct XTile {
         for (int n = 0; n < kAhead; ++n)
           v[n] = p[n] != nullptr && i < k ? *reinterpret_cast<const uint4*>(p[n] + i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < kAhead; ++n)
-          to[piece_index<F, kWidth>(i, (c0 + n) % kWidth)] = piece_order<F, T>(v[n]);
+        for (int n = 0; n < kAhead; ++n) {
+          if constexpr (W::kIs4) {
+            // the group's threads are neighbours (padded is whole warps)
+            const float2 a = MmaType<T>::unpack(v[n].x), b = MmaType<T>::unpack(v[n].y), c = MmaType<T>::unpack(v[n].z),
+                         d = MmaType<T>::unpack(v[n].w);
+            float sum = ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
+#pragma unroll
+            for (int o = W::kGroupK / 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (i % W::kGroupK == 0) sums[(c0 / kWidth * units * W::kSub + i / W::kGroupK) * 8 + n] = sum * Scaling<F, T>::kSum;
+          }
+          to[piece_index<F, kWidth>(i, n)] = piece_order<F, T>(v[n]);
+        }
       }
     }
     __syncthreads();
-    if constexpr (W::kIs4) {
-      const int lane = threadIdx.x & 31;
-      const int groups = live * units * W::kSub;
-#pragma unroll 1
-      for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
-        constexpr int kEach = W::kPieces / W::kSub;
-        float v = 0.0f;
-        if (lane < kWidth * 4) {
-#pragma unroll
-          for (int q = 0; q < kEach; ++q) {
-            const uint4 x = pieces[(g * kEach + q) * kWidth * 4 + (lane ^ piece_swap<F>(0, g % W::kSub * kEach + q))];
-            const float2 a = MmaType<T>::unpack(x.x), b = MmaType<T>::unpack(x.y), c = MmaType<T>::unpack(x.z),
-                         d = MmaType<T>::unpack(x.w);
-            v += ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
-          }
-        }
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
-        using S = Scaling<F, T>;
-        v = v * S::kSum * (1.0f / S::kX);
-        if ((lane & 3) == 0) sums[g * 8 + (lane >> 2)] = v;
-      }
-      __syncthreads();
-    }
   }
 
   // acc[b] += the step's rows times the columns of block b < NBL, over unit u.
@@ -350,6 +341,7 @@ struct XTile {
   template <int NBL, typename Scales>
   __device__ __forceinline__ void consume(float (&acc)[NB][4], uint32_t (&w)[2][4], int u, Scales scales) const {
     using M = MmaType<T>;
+    constexpr bool kApart = Scaling<F, T>::kApart;
     const int lane = threadIdx.x & 31;
     const uint4* at = pieces + u * kUnitPieces;
     auto piece = [&](int b, int j) -> uint4 {
@@ -371,7 +363,7 @@ struct XTile {
       }
 #pragma unroll
       for (int i = 0; i < W::kSub; ++i) {
-        float part[NBL][4] = {}, high[NBL][4] = {};
+        float part[NBL][4] = {}, odd[NBL][4] = {};
 #pragma unroll
         for (int q = 0; q < W::kPieces / W::kSub; ++q) {
           const int j = i * (W::kPieces / W::kSub) + q;
@@ -397,7 +389,7 @@ struct XTile {
           for (int b = 0; b < NBL; ++b) {
             const uint4 x = piece(b, j);
             M::mma(part[b], a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
-            M::mma(high[b], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
+            M::mma(kApart ? odd[b] : part[b], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
           }
         }
         float s[2], z[2];
@@ -405,7 +397,8 @@ struct XTile {
 #pragma unroll
         for (int b = 0; b < NBL; ++b) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n) part[b][n] = W::kIs4 ? fmaf(high[b][n], 1.0f / 16, part[b][n]) : part[b][n] + high[b][n];
+          for (int n = 0; n < 4; ++n)
+            if (kApart) part[b][n] = fmaf(odd[b][n], 1.0f / 16, part[b][n]);
           if constexpr (W::kIs4) {
             const float2 x = *reinterpret_cast<const float2*>(sums + ((b * units + u) * W::kSub + i) * 8 + 2 * (lane & 3));
 #pragma unroll

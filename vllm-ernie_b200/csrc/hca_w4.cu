@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   const int tiles = (a.n + 15) / 16, per_cta = kWarps / g.warps;
   const int t0 = blockIdx.y * X::kColumns;
   const int columns = min(X::kColumns, a.tokens - t0), live = (columns + kWidth - 1) / kWidth;
-  W4Tiles<F, T> src{a, static_cast<int>(blockIdx.x) * per_cta + g.id, static_cast<int>(gridDim.x) * per_cta, a.k / W::kGroupK};
+  W4Tiles<F, T> src{a, static_cast<int>(blockIdx.x + g.id * gridDim.x), static_cast<int>(gridDim.x) * per_cta, a.k / W::kGroupK};
 
   pdl_wait_and_release();
   TileStream<F, T> stream;
@@ -98,20 +98,22 @@ bool launch(W4Args a, cudaStream_t s, int& rc) {
   const int units = WTraits<F>::units(a.k), tiles = cdiv(a.n, 16), sms = device_sm_count();
   const int64_t columns = XTile<F, T, NB, kWidth>::bytes(units) + TileSums<NB>::bytes(kWarps);
   auto scales = [&](int warps) { return ScaleTile<F>::bytes(units, a.zeros != nullptr, warps, kWarps); };
-  // Warps to a tile: as few as leave every SM's groups four tiles each and
-  // room for the scales, but at least one quad a warp.  Few warps mean long
-  // runs between reductions, many that a short matrix still fills the machine.
-  a.group_warps = 1;
-  while (a.group_warps < kWarps && 8 * a.group_warps <= units &&
-         (tiles < 4ll * sms * (kWarps / a.group_warps) || columns + scales(a.group_warps) > kSmem))
-    a.group_warps *= 2;
+  // Warps to a tile: the number that makes the longest warp's work shortest,
+  // a tile's end (its sums meet) costing about what a quad of units does; as
+  // few as the room for scales allows of several.
+  a.group_warps = 0;
+  int64_t best = INT64_MAX;
+  for (int gw = 1; gw <= kWarps && 4 * gw <= units; gw *= 2) {
+    const int64_t cost = static_cast<int64_t>(cdiv(tiles, sms * (kWarps / gw))) * (cdiv(units, 4 * gw) + 1);
+    if (cost < best && columns + scales(gw) <= kSmem) best = cost, a.group_warps = gw;
+  }
+  if (a.group_warps == 0) return false;
   const int64_t smem = columns + scales(a.group_warps);
-  if (smem > kSmem) return false;
   static bool done[kMaxDevices] = {};
   rc = set_func_attr_once(w4_linear_kernel<F, T, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
   if (rc == HCA_OK) {
     rc = launch_pdl(w4_linear_kernel<F, T, NB, kWidth>,
-                    dim3(std::min(sms, cdiv(tiles, kWarps / a.group_warps)), cdiv(a.tokens, NB * kWidth)),
+                    dim3(std::min(sms, tiles), cdiv(a.tokens, NB * kWidth)),
                     dim3(kWarps * 32), static_cast<size_t>(smem), s, a);
   }
   return true;
