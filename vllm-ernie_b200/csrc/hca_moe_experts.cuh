@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Plan<NB * kWidth> pl;
   extern __shared__ __align__(16) uint8_t smem[];
   build_plan(pl, p);
-  TileStream<F, __nv_bfloat16> stream;
+  TileStream<F, __nv_bfloat16, WTraits<F>::step(NB)> stream;
   const int room = static_cast<int>(X::bytes(WTraits<F>::units(max(p.hidden, max(p.inner, p.shared_inner)))));
   uint8_t* sums = smem + room;
   TileSums<NB> ts(sums);
@@ -458,9 +458,17 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
 
 template <int F>
 int moe_experts_pass(const MoePass& p, const MoeWeights& w, cudaStream_t s) {
-  // Columns of an entry: as many as an expert may get and shared memory holds.
+  // Columns of an entry, where shared memory holds them: two blocks of eight if
+  // an expert gets more than eight tokens on average, or all tokens fit and it
+  // gets more than two; else one, which an expert with more tokens passes
+  // several times (at 64 tokens, four an expert, 188 us for 226 with 4-bit
+  // weights, 96 for 106 with e4m3; at 12 tokens, three an expert, 40 for 34 and
+  // 47 for 41).  bf16 weights, with nothing to unpack, gain from two blocks
+  // whenever there are more than eight tokens (58 us for 47 at 12 tokens).
   int rc = HCA_OK;
-  if (p.tokens > 8 && moe::launch<F, 2, 8>(p, w, s, rc)) return rc;
+  const int64_t pairs = static_cast<int64_t>(p.tokens) * p.routing.top_k;
+  const bool many = F == kWBf16 || pairs > static_cast<int64_t>(p.routing.experts) * (p.tokens <= 16 ? 2 : 8);
+  if (p.tokens > 8 && many && moe::launch<F, 2, 8>(p, w, s, rc)) return rc;
   if (p.tokens > 4 && moe::launch<F, 1, 8>(p, w, s, rc)) return rc;
   if (p.tokens > 2 && moe::launch<F, 1, 4>(p, w, s, rc)) return rc;
   if (moe::launch<F, 1, 2>(p, w, s, rc)) return rc;

@@ -65,6 +65,9 @@ struct WTraits {
   __host__ __device__ static constexpr int64_t row_bytes(int64_t k) {
     return F == kWBf16 ? 2 * k : F == kWFp8 ? k : k / 2;
   }
+  // units that a warp has on its way: with two blocks of columns and 4-bit
+  // codes four and the sums would not fit a thread's 128 registers (8 % slower)
+  static constexpr int step(int blocks) { return kIs4 && blocks > 1 ? 2 : 4; }
   // units of rows of k, in whole quads
   __host__ __device__ static constexpr int units(int k) { return (k + 4 * kUnitK - 1) / (4 * kUnitK) * 4; }
 };
@@ -471,13 +474,13 @@ struct TileRows {
 // consumed, source.zeros whether there are zero points (4-bit only).  Each is
 // asked for the tiles in order.  finish(i, sums) may move xt to the next tile's
 // columns.
-template <int F, typename T>
+template <int F, typename T, int kStep>
 struct TileStream {
   using W = WTraits<F>;
   struct Unit {
     uint32_t w[2][4];
     float s[2];  // e4m3
-  } quad[4];
+  } quad[kStep];
   TileRows at;  // of the tile whose units are loaded next
   ScaleTile<F> sc;
   int k, u0, u1, count, g0, g1;
@@ -488,7 +491,7 @@ struct TileStream {
   __device__ __forceinline__ void load(const TileRows& from, int u) {
     const int last = static_cast<int>(W::row_bytes(k)) - 16 * (1 + (static_cast<int>(threadIdx.x) & 3));
 #pragma unroll
-    for (int d = 0; d < 4; ++d) load_unit<kWhole>(quad[d], from, u, d, last);
+    for (int d = 0; d < kStep; ++d) load_unit<kWhole>(quad[d], from, u, d, last);
   }
   template <bool kWhole>
   __device__ __forceinline__ void load_unit(Unit& to, const TileRows& from, int u, int d, int last) const {
@@ -553,14 +556,14 @@ struct TileStream {
         }
       }
 #pragma unroll 1
-      for (int u = u0; u < u1; u += 4) {
+      for (int u = u0; u < u1; u += kStep) {
         // the quad after this one: the tile's next, or the next tile's first
         // (after the last tile its own first again, which nothing reads)
-        const bool ends = u + 4 >= u1;
+        const bool ends = u + kStep >= u1;
         if (ends && i + 1 < count) at = source.rows(i + 1);
-        const int next = ends ? u0 : u + 4;
+        const int next = ends ? u0 : u + kStep;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
+        for (int d = 0; d < kStep; ++d) {
           xt.template consume<NBL>(acc, quad[d].w, u + d, [&](int j, float (&s)[2], float (&z)[2]) {
             if constexpr (W::kIs4) {
               const int n = (u + d) * W::kSub + j;

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   W4Tiles<F, T> src{a, static_cast<int>(blockIdx.x + g.id * gridDim.x), static_cast<int>(gridDim.x) * per_cta, a.k / W::kGroupK};
 
   pdl_wait_and_release();
-  TileStream<F, T> stream;
+  TileStream<F, T, WTraits<F>::step(NB)> stream;
   stream.start(a.k, g, src.first < tiles ? (tiles - src.first + src.stride - 1) / src.stride : 0,
              smem + X::bytes(units) + TileSums<NB>::bytes(kWarps), src);
   const T* x = static_cast<const T*>(a.x) + t0 * a.x_stride;
