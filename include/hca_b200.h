@@ -50,7 +50,8 @@ int hca_version(void);
 /* Device error word of the current device (synchronous read): non-zero if a
  * kernel gave up on a bounded wait (bit 0 loader, 1 dequant, 2 MMA, 3
  * softmax of hca_sparse_decode; bit 4 the streamed many-token path of
- * hca_qnorm_rope_kv_insert, bit 5 that of hca_vha_inv_rope_fp8_quant).
+ * hca_qnorm_rope_kv_insert, bit 5 that of hca_vha_inv_rope_fp8_quant, bit 6 the
+ * steps of hca_moe_experts and hca_moe_decode).
  * clear != 0 resets it to zero. */
 int hca_device_error(int32_t* value, int32_t clear);
 
@@ -447,7 +448,9 @@ int hca_fp8_grouped_gemm(void* out, int64_t out_stride_tok, int64_t out_stride_g
  * aligned, the low nibble of a byte the even k; scales [N, K / g] of x's
  * type; zeros [N, K / g] whole numbers 0..255, NULL = 8 everywhere.
  * g = group_size 32, 64 or 128, dividing K.  Products and sums in fp32, one
- * rounding.  Any T is right; the weights are read again for every 32 rows. */
+ * rounding.  Any T is right; the weights are read again for every 16 rows
+ * (fewer, where shared memory does not hold 16 rows of x).
+ * q starts on 16 bytes, scales and zeros on 4; out must not overlap x. */
 int hca_w4_linear(void* out, int64_t out_stride, const void* x, int64_t x_stride, const uint8_t* q,
                   const void* scales, const uint8_t* zeros, int32_t num_tokens, int32_t n, int32_t k,
                   int32_t group_size, int32_t is_fp16, void* stream);
@@ -478,8 +481,10 @@ int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride,
  *   out[t] = sum_j weights[t, j] * W2_e (silu(W1_e x_t) * (W3_e x_t)), e = ids[t, j]
  * plus the shared expert's W2 (silu(W1 x) * (W3 x)) where shared_inner > 0.
  * w13 [E, 2 I, H] (W1 over W3), w2 [E, H, I], shared13 [2 Is, H], shared2
- * [H, Is], all of one format, contiguous, 16-byte aligned.  ids outside
- * [0, E) are skipped; an id may repeat.  A row whose token_mask byte is 0
+ * [H, Is], all of one format (zero points for all or none of a product's
+ * matrices), contiguous, 16-byte aligned, scales and zero points 4-byte
+ * aligned.  ids outside
+ * [0, E) are skipped; an id that repeats in a row counts with its weights' sum.  A row whose token_mask byte is 0
  * takes no part and its out is 0.  I, Is and H multiples of 32 (and of the
  * group).  The gated product is rounded to bf16 once, with its weight in it;
  * everything else is summed in fp32.  Any T; passes of 64 tokens.

@@ -689,3 +689,174 @@ def test_logit_penalties_refuse(change):
         x = torch.zeros((100, 3), device=DEV).T
     with pytest.raises(ValueError):
         _ops().apply_logit_penalties(x, ids, **how)
+
+
+# ---------------------------------------------------------------------------
+# the ends of the ranges
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("tokens,n,k", [
+    (3, 70, 640), (4, 16, 8192), (5, 100, 4224), (7, 33, 128), (10, 40, 8192),
+    (8, 50, 16384),   # shared memory holds four rows: two passes over the weights
+    (11, 20, 16384),
+    (3, 24, 32768),   # two rows
+    (1, 40, 65536),   # pieces of a row
+    (11, 2400, 61568),
+])
+def test_w4_linear_few_rows_and_long_ones(tokens, n, k, group, zeros, dtype):
+    gen = _gen(tokens + n + k)
+    x = torch.randn((tokens, k), generator=gen, device=DEV).to(dtype)
+    q, s, z, w = _w4((n, k), group, zeros, gen, dtype)
+    got = _ops().w4_linear(x, q, s, z)
+    xd = x.double()
+    size = xd.abs() @ (s.double().repeat_interleave(group, 1) * 15).T
+    _within(got, xd @ w.T, U[dtype] * (xd @ w.T).abs() + 2.0 ** -22 * k * size + 1e-6)
+
+
+@pytest.mark.parametrize("dtype,exponents", [(torch.bfloat16, [-60, -20, 0, 20, 40]), (torch.float16, [-14, -7, 0, 7, 11])])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_w4_linear_magnitudes(group, dtype, exponents):
+    """Rows of very different sizes, each exact to its own size."""
+    gen = _gen(31)
+    x = torch.randn((len(exponents), 1280), generator=gen, device=DEV).clamp(-4, 4)
+    x = (x * torch.exp2(torch.tensor(exponents, device=DEV, dtype=torch.float32)).unsqueeze(1)).to(dtype)
+    q, s, z, _ = _w4((90, 1280), group, True, gen, dtype)
+    z.copy_(torch.randint(0, 256, z.shape, generator=gen, device=DEV))  # any byte
+    s /= 64  # keeps fp16 results in range
+    w = (q.long().unsqueeze(-1) >> torch.tensor([0, 4], device=DEV) & 15).flatten(-2).double()
+    w = (w - z.double().repeat_interleave(group, 1)) * s.double().repeat_interleave(group, 1)
+    s64 = s.double().repeat_interleave(group, 1)
+    got, ref = _ops().w4_linear(x, q, s, z), x.double() @ w.T
+    size = x.double().abs() @ (s64 * 255).T
+    least = 2.0 ** -25 if dtype is torch.float16 else 0.0  # half a step of the smallest results
+    # the group sum of x and its product with the zero point round as well
+    _within(got, ref, U[dtype] * ref.abs() + 2.0 ** -22 * 1280 * size + least)
+
+
+def test_w4_linear_refuses_misaligned_scales_and_overlapping_rows():
+    from vllm_ernie_b200 import HcaError
+
+    gen = _gen(32)
+    x, (q, s, _, _) = torch.zeros((1, 96), device=DEV, dtype=torch.bfloat16), _w4((3, 96), 32, False, gen)
+    odd = torch.ones(10, device=DEV, dtype=torch.bfloat16)[1:].view(3, 3)  # two bytes past a word
+    with pytest.raises(HcaError) as e:
+        _ops().w4_linear(x, q, odd)
+    assert e.value.status == -1
+    two = torch.zeros((2, 96), device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        _ops().w4_linear(two, q, s, out=torch.zeros((1, 3), device=DEV, dtype=torch.bfloat16).expand(2, 3))
+
+
+@pytest.mark.parametrize("kind", FORMATS)
+@pytest.mark.parametrize("tokens,hidden,inner,shared", [
+    (9, 8192, 128, 256),    # shared memory holds one block of columns
+    (16, 512, 8192, 0),
+    (6, 16384, 128, 128),   # four columns
+    (12, 8192, 1024, 128),
+])
+def test_moe_experts_long_rows(tokens, hidden, inner, shared, kind):
+    gen = _gen(tokens + hidden)
+    x = torch.randn((tokens, hidden), generator=gen, device=DEV).to(torch.bfloat16)
+    stack, w13, w2 = _stack(kind, (3,), hidden, inner, gen)
+    one, a, b = _stack(kind, (), hidden, shared, gen) if shared else (None, None, None)
+    ids = torch.rand((tokens, 3), generator=gen, device=DEV).argsort(1)[:, :2].int().contiguous()
+    weights = torch.rand((tokens, 2), generator=gen, device=DEV)
+    got = _ops().moe_experts(x, ids, weights, stack, shared=one)
+    ref, size = _experts_ref(x, ids, weights, w13, w2, shared=(a, b) if shared else None)
+    _within(got, ref, _moe_bound(ref, size, hidden + 2 * inner + shared))
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 16, 17, 64])
+@pytest.mark.parametrize("experts,k", [(129, 6), (512, 16)])
+def test_moe_decode_of_many_experts_is_route_then_experts(experts, k, tokens):
+    ops, gen = _ops(), _gen(33)
+    x = torch.randn((tokens, 256), generator=gen, device=DEV).to(torch.bfloat16)
+    wr = torch.randn((experts, 256), generator=gen, device=DEV) * 0.1
+    stack, _, _ = _stack("w4-32", (experts,), 256, 64, gen)
+    shared, _, _ = _stack("w4-32", (), 256, 96, gen)
+    ids, weights = ops.moe_route(x, wr, k)
+    got = ops.moe_decode(x, wr, stack, k, shared=shared)
+    assert torch.equal(got, ops.moe_experts(x, ids, weights, stack, shared=shared))
+
+
+def test_moe_result_does_not_depend_on_the_batchs_other_tokens():
+    ops, gen = _ops(), _gen(34)
+    x = torch.randn((11, 512), generator=gen, device=DEV).to(torch.bfloat16)
+    wr = torch.randn((24, 512), generator=gen, device=DEV) * 0.1
+    stack, _, _ = _stack("w4-64z", (24,), 512, 192, gen)
+    first = ops.moe_decode(x, wr, stack, 3)
+    other = torch.randn((11, 512), generator=gen, device=DEV).to(torch.bfloat16)
+    other[7] = x[2]
+    assert torch.equal(ops.moe_decode(other, wr, stack, 3)[7], first[2])
+
+
+@pytest.mark.parametrize("change", ["one", "other", "overlapping"])
+def test_moe_refuses_half_a_format(change):
+    """Zero points for the experts and none for the shared one, or the other
+    way round; rows of a result on top of each other."""
+    ops, gen = _ops(), _gen(35)
+    x = torch.randn((3, 128), generator=gen, device=DEV).to(torch.bfloat16)
+    wr = torch.randn((8, 128), generator=gen, device=DEV)
+    stack, _, _ = _stack("w4-64z", (8,), 128, 64, gen)
+    shared, _, _ = _stack("w4-64z", (), 128, 64, gen)
+    out = None
+    if change == "one":
+        shared = shared._replace(z13=None)
+    elif change == "other":
+        stack = stack._replace(z2=None)
+    else:
+        out = torch.zeros((1, 128), device=DEV, dtype=torch.bfloat16).expand(3, 128)
+    with pytest.raises(ValueError):
+        ops.moe_decode(x, wr, stack, 2, shared=shared, out=out)
+
+
+@pytest.mark.parametrize("zeros", ["z13", "z2"])
+def test_moe_zero_points_of_one_product(zeros):
+    ops, gen = _ops(), _gen(36)
+    x = torch.randn((4, 256), generator=gen, device=DEV).to(torch.bfloat16)
+    q13, s13, z13, w13 = _w4((5, 384, 256), 64, zeros == "z13", gen)
+    q2, s2, z2, w2 = _w4((5, 256, 192), 64, zeros == "z2", gen)
+    ids = torch.randint(0, 5, (4, 1), generator=gen, device=DEV, dtype=torch.int32)
+    weights = torch.rand((4, 1), generator=gen, device=DEV)
+    got = ops.moe_experts(x, ids, weights, ops.MoEWeights(q13, q2, s13, s2, z13, z2))
+    ref, size = _experts_ref(x, ids, weights, w13, w2)
+    _within(got, ref, _moe_bound(ref, size, 256 + 192))
+
+
+@pytest.mark.parametrize("shift", [2, 4, 6, 8])
+def test_4_bit_scales_that_start_off_16_bytes(shift):
+    """Rows of whole 16 bytes whose arrays start elsewhere."""
+    ops, gen = _ops(), _gen(37)
+
+    def moved(v, by):
+        flat = torch.zeros(v.numel() + by, device=DEV, dtype=v.dtype)
+        flat[by:] = v.flatten()
+        return flat[by:].view(v.shape)
+
+    x = torch.randn((3, 4096), generator=gen, device=DEV).to(torch.bfloat16)
+    q, s, z, _ = _w4((100, 4096), 32, True, gen)
+    assert torch.equal(ops.w4_linear(x, q, moved(s, shift), moved(z, 2 * shift)), ops.w4_linear(x, q, s, z))
+    x = x[:, :1024].contiguous()
+    stack, _, _ = _stack("w4-64z", (5,), 1024, 512, gen)
+    one, _, _ = _stack("w4-64z", (), 1024, 512, gen)
+    wr = torch.randn((5, 1024), generator=gen, device=DEV) * 0.1
+    first = ops.moe_decode(x, wr, stack, 2, shared=one)
+
+    def off(w):
+        return w._replace(s13=moved(w.s13, shift), s2=moved(w.s2, shift), z13=moved(w.z13, 2 * shift), z2=moved(w.z2, 2 * shift))
+
+    assert torch.equal(ops.moe_decode(x, wr, off(stack), 2, shared=one), first)
+    assert torch.equal(ops.moe_decode(x, wr, stack, 2, shared=off(one)), first)
+
+
+def test_logit_penalties_refuse_rows_on_top_of_each_other():
+    x = torch.zeros((1, 64), device=DEV).expand(3, 64)
+    with pytest.raises(ValueError):
+        _ops().apply_logit_penalties(x, frequency=torch.zeros(3, device=DEV))
+
+
+def test_no_wait_gave_up():
+    assert _ops().device_error() == 0

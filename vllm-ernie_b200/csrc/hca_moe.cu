@@ -200,6 +200,9 @@ int check_weights(const MoeWeights& w, int format, int group, int hidden, int in
   if (rc == HCA_OK) rc = check_matrix(w.w2, format);
   if (rc == HCA_OK && shared_inner > 0) rc = check_matrix(w.shared13, format);
   if (rc == HCA_OK && shared_inner > 0) rc = check_matrix(w.shared2, format);
+  // zero points are a part of the format that both share
+  HCA_CHECK_ARG(shared_inner == 0 || ((w.w13.zero == nullptr) == (w.shared13.zero == nullptr) &&
+                                      (w.w2.zero == nullptr) == (w.shared2.zero == nullptr)));
   return rc;
 }
 

@@ -246,7 +246,15 @@ struct Product {
     }
     return t;
   }
-  __device__ __forceinline__ bool zeros() const { return (kUp ? w.w13.zero : w.w2.zero) != nullptr || (kUp ? w.shared13.zero : w.shared2.zero) != nullptr; }
+  __device__ __forceinline__ bool zeros() const { return (kUp ? w.w13.zero : w.w2.zero) != nullptr; }
+  __device__ __forceinline__ bool rows_wide() const {
+    const MoeMatrix &m = kUp ? w.w13 : w.w2, &one = kUp ? w.shared13 : w.shared2;
+    const int groups = k_of(first_entry) / W::kGroupK;
+    // of one segment all entries are the experts' or the shared one's
+    return dense || first_entry < pl.routed ? scales_wide(m.scale, m.zero, groups) &&
+                                                  (!dense || p.shared_inner == 0 || scales_wide(one.scale, one.zero, groups))
+                                            : scales_wide(one.scale, one.zero, groups);
+  }
   __device__ __forceinline__ WScales scales_of(const Place& at, int r) const {
     int64_t e;
     const MoeMatrix& m = matrix(at, e);
@@ -378,7 +386,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   {
     Product<F, NB, kWidth, false> down(p, w, pl, smem, room, scales, shape.down_warps, false);
     bool more = down.start(stream);
-    if (!grid_wait(p.barrier, 1, p.error)) return;
+    if (!grid_wait(p.barrier, 1, p.error)) {
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
+      return;
+    }
     while (more) {
       down.run(stream, ts);
       more = down.start(stream);
@@ -412,9 +423,13 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   using W = WTraits<F>;
   const int sms = device_sm_count();
   const int inner = std::max(p.inner, p.shared_inner);
+  // the shares of the work are counted in 32 bits: every pair an entry at most
+  const int64_t units = std::max(static_cast<int64_t>(inner / 8) * W::units(p.hidden),
+                                 static_cast<int64_t>(p.hidden / 16) * W::units(inner));
+  if (units * p.tokens * (p.routing.top_k + 1) > UINT32_MAX) return false;
   const int64_t columns = XTile<F, __nv_bfloat16, NB, kWidth>::bytes(W::units(std::max(p.hidden, inner))) +
                           TileSums<NB>::bytes(kWarps);
-  const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr || w.shared13.zero != nullptr || w.shared2.zero != nullptr;
+  const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr;
   auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
   // Warps to a tile: the number that makes the longest warp's work shortest (if
   // every pair chose another expert), a tile's end costing about what a quad of

@@ -221,11 +221,16 @@ struct WScales {
   const uint8_t *scale, *scale_end;
   const uint8_t *zero, *zero_end;  // null: 8 everywhere
 };
+// Whether rows of `groups` scales start on 16 bytes and their zero points on 8.
+__device__ __forceinline__ bool scales_wide(const void* scale, const void* zero, int groups) {
+  return ((reinterpret_cast<uintptr_t>(scale) | 2 * reinterpret_cast<uintptr_t>(zero) | 2 * groups) & 15) == 0;
+}
 
 // Scales and zero points of a warp's share of a tile, in shared memory, two
 // tiles in turn.  If every row's share begins and ends on 16 bytes (wide), it
 // is copied in pieces of 16 (zero points 8); else whole words around it are,
-// and it starts 0..3 bytes into the first.
+// and it starts 0..3 bytes into the first.  The former depends on the arrays'
+// first bytes, on the groups of a whole row of theirs and on the share's ends.
 template <int F>
 struct ScaleTile {
   using W = WTraits<F>;
@@ -245,11 +250,11 @@ struct ScaleTile {
     return W::kIs4 ? 32ll * block_warps * row_pitch(share(units, group_warps), zeros) : 0;
   }
 
-  __device__ __forceinline__ void init(uint8_t* smem, int units, bool zeros, int warps, int groups, int g0, int g1) {
+  __device__ __forceinline__ void init(uint8_t* smem, int units, bool zeros, int warps, bool rows_wide, int g0, int g1) {
     const int n = share(units, warps);
     zero_at = zero_offset(n), pitch = row_pitch(n, zeros);
     base = smem + (threadIdx.x >> 5) * 32 * pitch;
-    wide = ((groups | g0 | g1 | n) & 7) == 0;
+    wide = rows_wide && ((g0 | g1 | n) & 7) == 0;
   }
   __device__ __forceinline__ uint8_t* row(int i, int r) const { return base + ((i & 1) * 16 + r) * pitch; }
   // Starts the copy of groups [g0, g1) of the lane's row of tile `i`: lanes l
@@ -471,7 +476,8 @@ struct TileRows {
 // A warp's share of a run of tiles.  `source` knows the tiles: source.rows(i)
 // are the lane's rows of the group's i-th tile, source.scales(i, row) tells
 // where the scales of a row of it are and source.here the same for the tile now
-// consumed, source.zeros whether there are zero points (4-bit only).  Each is
+// consumed, source.zeros whether there are zero points and source.rows_wide
+// what scales_wide says of the arrays (4-bit only).  Each is
 // asked for the tiles in order.  finish(i, sums) may move xt to the next tile's
 // columns.
 template <int F, typename T, int kStep>
@@ -521,7 +527,7 @@ struct TileStream {
     }
     if constexpr (W::kIs4) {
       g0 = min(u0 * W::kSub, k / W::kGroupK), g1 = min(u1 * W::kSub, k / W::kGroupK);
-      sc.init(smem, units, source.zeros(), g.warps, k / W::kGroupK, g0, g1);
+      sc.init(smem, units, source.zeros(), g.warps, source.rows_wide(), g0, g1);
       __syncwarp();  // the last run's scales have been read
       fetch_scales(0, source);
       fetch_scales(1, source);

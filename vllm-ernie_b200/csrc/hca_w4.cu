@@ -17,6 +17,9 @@ namespace {
 constexpr int kWarps = 16;
 // shared memory of a CTA: x and the tile sums
 constexpr int64_t kSmem = 227 * 1024;
+// Rows of x too long for that are taken in pieces of 4096, two warps a tile:
+// eight tiles use a piece while it is there (four times the bytes of eight rows).
+constexpr int kLongK = 4096, kLongWarps = 2;
 
 struct W4Args {
   void* out;
@@ -36,6 +39,7 @@ struct W4Tiles {
   using W = WTraits<F>;
   const W4Args& a;
   int first, stride, groups;
+  int k0 = 0;  // first k of the piece
 
   __device__ __forceinline__ int64_t row(int i, int r) const {
     return min((first + i * stride) * 16 + r, a.n - 1);  // rows past the end are read again, not stored
@@ -44,12 +48,14 @@ struct W4Tiles {
     const int lane = threadIdx.x & 31;
     TileRows t;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) t.data[r] = a.q + (lane & 3) * 16 + row(i, (lane >> 2) + 8 * r) * W::row_bytes(a.k);
+    for (int r = 0; r < 2; ++r)
+      t.data[r] = a.q + (lane & 3) * 16 + row(i, (lane >> 2) + 8 * r) * W::row_bytes(a.k) + W::row_bytes(k0);
     return t;
   }
   __device__ __forceinline__ bool zeros() const { return a.zeros != nullptr; }
+  __device__ __forceinline__ bool rows_wide() const { return scales_wide(a.scales, a.zeros, groups); }
   __device__ __forceinline__ WScales here(int i, int r) const {
-    const int64_t at = row(i, r) * groups, all = static_cast<int64_t>(a.n) * groups;
+    const int64_t at = row(i, r) * groups + k0 / W::kGroupK, all = static_cast<int64_t>(a.n) * groups;
     const uint8_t* s = static_cast<const uint8_t*>(a.scales);
     return {s + 2 * at, s + 2 * all, a.zeros == nullptr ? nullptr : a.zeros + at, a.zeros + all};
   }
@@ -92,6 +98,64 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   else stream.template run<NB>(xt, g, ts, acc, src, finish);
 }
 
+// The same for rows of any length: a group holds one tile at a time, for which
+// the pieces of x come into shared memory in turn.
+template <int F, typename T>
+__global__ void __launch_bounds__(kWarps * 32, 1) w4_long_kernel(W4Args a) {
+  using W = WTraits<F>;
+  using X = XTile<F, T, 1, 8>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const TileGroup g(kLongWarps);
+  constexpr int per_cta = kWarps / kLongWarps, units = W::units(kLongK);
+  TileSums<1> ts(smem + X::bytes(units));
+  float* total = reinterpret_cast<float*>(smem + X::bytes(units) + TileSums<1>::bytes(kWarps)) + g.id * 128;
+  uint8_t* scales = smem + X::bytes(units) + TileSums<1>::bytes(kWarps) + per_cta * 512;
+  const int tiles = (a.n + 15) / 16, t0 = blockIdx.y * X::kColumns, columns = min(X::kColumns, a.tokens - t0);
+  const T* x = static_cast<const T*>(a.x) + t0 * a.x_stride;
+  pdl_wait_and_release();
+#pragma unroll 1
+  for (int64_t first = blockIdx.x; first < tiles; first += static_cast<int64_t>(gridDim.x) * per_cta) {
+    const int64_t tile = first + g.id * gridDim.x;
+    const bool mine = tile < tiles;
+    W4Tiles<F, T> src{a, static_cast<int>(mine ? tile : 0), 0, a.k / W::kGroupK};
+#pragma unroll 1
+    for (; src.k0 < a.k; src.k0 += kLongK) {
+      const int k = min(kLongK, a.k - src.k0);
+      TileStream<F, T, W::step(1)> stream;
+      stream.start(k, g, mine, scales, src);
+      __syncthreads();  // the last piece has been read
+      X xt(smem, W::units(k));
+      xt.stage(k, columns, 1, [&](int col) { return x + col * a.x_stride + src.k0; });
+      float acc[1][4] = {};
+      // a thread meets the same sums each time
+      stream.template run<1>(xt, g, ts, acc, src, [&](int, const float* sums) {
+#pragma unroll 1
+        for (int j = g.thread(); j < 128; j += g.threads()) {
+          const int64_t row = tile * 16 + (j & 15);
+          const int col = j >> 4;
+          float v = TileSums<1>::sum(sums, g, j & 15, 0, col) * Scaling<F, T>::kOut;
+          if (src.k0 > 0) v += total[j];
+          if (src.k0 + k < a.k) total[j] = v;
+          else if (row < a.n && col < columns) static_cast<T*>(a.out)[(t0 + col) * a.out_stride + row] = MmaType<T>::from_float(v);
+        }
+      });
+    }
+  }
+}
+
+template <int F, typename T>
+int launch_long(const W4Args& a, cudaStream_t s) {
+  constexpr int units = WTraits<F>::units(kLongK);
+  const int tiles = cdiv(a.n, 16), sms = device_sm_count();
+  const int64_t smem = XTile<F, T, 1, 8>::bytes(units) + TileSums<1>::bytes(kWarps) + kWarps / kLongWarps * 512 +
+                       ScaleTile<F>::bytes(units, a.zeros != nullptr, kLongWarps, kWarps);
+  static bool done[kMaxDevices] = {};
+  const int rc = set_func_attr_once(w4_long_kernel<F, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
+  if (rc != HCA_OK) return rc;
+  return launch_pdl(w4_long_kernel<F, T>, dim3(std::min(sms, tiles), cdiv(a.tokens, 8)), dim3(kWarps * 32),
+                    static_cast<size_t>(smem), s, a);
+}
+
 // Launches with NB blocks of kWidth columns if shared memory holds them.
 template <int F, typename T, int NB, int kWidth>
 bool launch(W4Args a, cudaStream_t s, int& rc) {
@@ -128,7 +192,7 @@ int by_rows(const W4Args& a, cudaStream_t s) {
   if (a.tokens > 4 && launch<F, T, 1, 8>(a, s, rc)) return rc;
   if (a.tokens > 2 && launch<F, T, 1, 4>(a, s, rc)) return rc;
   if (launch<F, T, 1, 2>(a, s, rc)) return rc;
-  return HCA_E_UNSUPPORTED;
+  return launch_long<F, T>(a, s);
 }
 
 template <typename T>

@@ -555,7 +555,7 @@ def _refuse(what: str):
 def _device_of(x: torch.Tensor, *ts: torch.Tensor | None) -> int:
     """The device of all the tensors, which has to be the current one."""
     dev = x.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != torch._C._cuda_getDevice():
         _refuse("libhca_b200 ops take CUDA tensors of the current device")
     for t in ts:
         if t is not None and t.get_device() != dev:
@@ -567,38 +567,42 @@ def _stream(dev: int) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _rows_out(x: torch.Tensor, dev: int, t: int, n: int, out: torch.Tensor | None) -> torch.Tensor:
-    if out is None:
-        return x.new_empty((t, n))
-    if (out.get_device() != dev or out.dtype is not x.dtype or out.shape != (t, n) or (n > 1 and out.stride(1) != 1)):
-        _refuse(f"out must be {x.dtype} [{t}, {n}] with contiguous rows, on x's device")
-    return out
+def _rows_out(x: torch.Tensor, dev: int, t: int, n: int, out: torch.Tensor) -> int:
+    """Row stride of a caller's ``out``."""
+    if out.get_device() != dev or out.dtype is not x.dtype or out.shape != (t, n):
+        _refuse(f"out must be {x.dtype} [{t}, {n}] on x's device")
+    stride, inner = out.stride()
+    if (n > 1 and inner != 1) or (t > 1 and stride < n):
+        _refuse("out must have contiguous rows that do not overlap")
+    return stride
 
 
 def _check_rows(x: torch.Tensor) -> tuple[int, int, int, int]:
     """``(T, K, row stride, address)`` of a matrix whose rows start on 16 bytes."""
-    if x.dim() != 2:
-        _refuse("x must be [T, K]")
-    t, k = x.shape
+    try:
+        t, k = x.shape
+    except ValueError:
+        _refuse("x must be a matrix")
     stride, inner = x.stride()
     at = x.data_ptr()
-    if (k > 1 and inner != 1) or (t > 1 and stride % 8) or at % 16:
+    if (inner != 1 and k > 1) or (stride % 8 and t > 1) or at % 16:
         _refuse("x must have contiguous rows that start on 16 bytes")
     return t, k, stride if t > 1 else k + -k % 8, at
 
 
 def _check_w4(q, s, z, lead: tuple, n: int, k: int, dtype) -> int:
     """Group size of the 4-bit weights ``[*lead, n, k]``."""
-    if q.dtype is not _U8 or k % 2 or q.shape != (*lead, n, k // 2) or not q.is_contiguous():
-        _refuse(f"4-bit codes must be contiguous uint8 {[*lead, n, k // 2]}")
     shape = s.shape
-    if len(shape) != len(lead) + 2 or shape[-1] == 0 or k % shape[-1] or k // shape[-1] not in W4_GROUPS:
+    groups = shape[-1] if len(shape) else 0
+    if groups == 0 or k % groups or k // groups not in W4_GROUPS:
         _refuse(f"scales must be [..., N, K / group] for a group of {W4_GROUPS}")
-    if s.dtype is not dtype or shape[:-1] != (*lead, n) or not s.is_contiguous():
-        _refuse(f"scales must be contiguous {dtype} {[*lead, n, shape[-1]]}")
+    if q.dtype is not _U8 or q.shape != (*lead, n, k // 2) or not q.is_contiguous():
+        _refuse(f"4-bit codes must be contiguous uint8 {[*lead, n, k // 2]}")
+    if s.dtype is not dtype or shape != (*lead, n, groups) or not s.is_contiguous():
+        _refuse(f"scales must be contiguous {dtype} {[*lead, n, groups]}")
     if z is not None and (z.dtype is not _U8 or z.shape != shape or not z.is_contiguous()):
         _refuse("zero points must be contiguous uint8 of the scales' shape")
-    return k // shape[-1]
+    return k // groups
 
 
 def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
@@ -608,22 +612,28 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
     ``x`` ``[T, K]`` bf16 or fp16; ``qweight`` uint8 ``[N, K / 2]`` (low nibble
     = even k); ``scales`` ``[N, K / g]`` of x's type, g = 32, 64 or 128;
     ``zeros`` uint8 ``[N, K / g]`` (None: 8).  ``w = (q - zero) * scale``, sums
-    in fp32, one rounding to x's type.  Right for any T, made for up to 16 rows
-    (each 16 more read the weights again; a prompt's thousands belong on a dense
-    product)."""
+    in fp32, one rounding to x's type.  ``out`` must not overlap ``x``.  Right
+    for any T, made for up to 16 rows (each 16 more read the weights again; a
+    prompt's thousands belong on a dense product)."""
     dev = _device_of(x, qweight, scales, zeros)
     dtype = x.dtype
     if dtype is not _BF16 and dtype is not _FP16:
         _refuse(f"x must be bf16 or fp16, got {dtype}")
     t, k, stride, at = _check_rows(x)
-    if qweight.dim() != 2 or qweight.shape[0] == 0 or k == 0:
+    try:
+        n, _ = qweight.shape
+    except ValueError:
         _refuse("qweight must be [N, K / 2]")
-    n = qweight.shape[0]
+    if n == 0:
+        _refuse("qweight has no rows")
     group = _check_w4(qweight, scales, zeros, (), n, k, dtype)
-    out = _rows_out(x, dev, t, n, out)
+    if out is None:
+        out, out_stride = x.new_empty(t, n), n
+    else:
+        out_stride = _rows_out(x, dev, t, n, out)
     if t:
-        call("hca_w4_linear", out.data_ptr(), out.stride(0), at, stride, qweight.data_ptr(), scales.data_ptr(), _p(zeros), t,
-             n, k, group, dtype is _FP16, _stream(dev))
+        call("hca_w4_linear", out.data_ptr(), out_stride, at, stride, qweight.data_ptr(), scales.data_ptr(),
+             None if zeros is None else zeros.data_ptr(), t, n, k, group, dtype is _FP16, _stream(dev))
     return out
 
 
@@ -674,45 +684,57 @@ _MOE_FORMATS = {torch.bfloat16: 0, FP8: 1, torch.uint8: 2}
 def _moe_weights(w: MoEWeights, lead: tuple, hidden: int, dev: int) -> tuple[int, int, int, tuple]:
     """``(format, group, inner, addresses)`` of checked weights."""
     w13, w2, s13, s2, z13, z2 = w
-    for m in w:
-        if m is not None and m.get_device() != dev:
-            _refuse("expert weights must be on x's device")
     fmt = _MOE_FORMATS.get(w13.dtype, -1)
     if fmt < 0 or w2.dtype is not w13.dtype:
         _refuse("expert weights must be bf16, e4m3 or uint8 (4-bit codes), both alike")
+    if not w13.get_device() == w2.get_device() == dev:
+        _refuse("expert weights must be on x's device")
     shape = w13.shape
     if len(shape) != len(lead) + 2 or shape[-2] % 2 or shape[-2] == 0:
         _refuse(f"w13 must be {[*lead, '2 I', 'H']}")
     inner = shape[-2] // 2
-    if fmt == 2:
-        if s13 is None or s2 is None:
-            _refuse("4-bit experts need scales")
-        group = _check_w4(w13, s13, z13, lead, 2 * inner, hidden, _BF16)
-        if _check_w4(w2, s2, z2, lead, hidden, inner, _BF16) != group:
-            _refuse("w13 and w2 must have one group size")
-        return fmt, group, inner, (w13.data_ptr(), s13.data_ptr(), _p(z13), w2.data_ptr(), s2.data_ptr(), _p(z2))
-    if z13 is not None or z2 is not None:
-        _refuse("only 4-bit experts have zero points")
-    if shape != (*lead, 2 * inner, hidden) or w2.shape != (*lead, hidden, inner) or not (w13.is_contiguous() and w2.is_contiguous()):
-        _refuse(f"expert weights must be contiguous {[*lead, 2 * inner, hidden]} and {[*lead, hidden, inner]}")
     if fmt == 0:
         if s13 is not None or s2 is not None:
             _refuse("bf16 experts have no scales")
-    else:
+    elif s13 is None or s2 is None:
+        _refuse("e4m3 and 4-bit experts need scales")
+    elif not s13.get_device() == s2.get_device() == dev:
+        _refuse("expert weights must be on x's device")
+    zeros = None, None
+    if z13 is not None or z2 is not None:
+        if fmt != 2:
+            _refuse("only 4-bit experts have zero points")
+        for z in (z13, z2):
+            if z is not None and z.get_device() != dev:
+                _refuse("expert weights must be on x's device")
+        zeros = _p(z13), _p(z2)
+    if fmt == 2:
+        group = _check_w4(w13, s13, z13, lead, 2 * inner, hidden, _BF16)
+        if _check_w4(w2, s2, z2, lead, hidden, inner, _BF16) != group:
+            _refuse("w13 and w2 must have one group size")
+        return fmt, group, inner, (w13.data_ptr(), s13.data_ptr(), zeros[0], w2.data_ptr(), s2.data_ptr(), zeros[1])
+    if shape != (*lead, 2 * inner, hidden) or w2.shape != (*lead, hidden, inner) or not (w13.is_contiguous() and w2.is_contiguous()):
+        _refuse(f"expert weights must be contiguous {[*lead, 2 * inner, hidden]} and {[*lead, hidden, inner]}")
+    if fmt == 1:
         for s, n, k in ((s13, 2 * inner, hidden), (s2, hidden, inner)):
-            if s is None or s.dtype is not _FP32 or s.shape != (*lead, -(-n // 128), -(-k // 128)) or not s.is_contiguous():
+            if s.dtype is not _FP32 or s.shape != (*lead, -(-n // 128), -(-k // 128)) or not s.is_contiguous():
                 _refuse(f"block scales must be contiguous fp32 {[*lead, -(-n // 128), -(-k // 128)]}")
-    return fmt, 0, inner, (w13.data_ptr(), _p(s13), None, w2.data_ptr(), _p(s2), None)
+        return fmt, 0, inner, (w13.data_ptr(), s13.data_ptr(), None, w2.data_ptr(), s2.data_ptr(), None)
+    return fmt, 0, inner, (w13.data_ptr(), None, None, w2.data_ptr(), None, None)
 
 
-def _moe_args(x, dev: int, hidden: int, experts: MoEWeights, shared: MoEWeights | None):
+_NO_SHARED = (None,) * 6
+
+
+def _moe_args(hidden: int, dev: int, experts: MoEWeights, shared: MoEWeights | None):
     """Checked ``(format, group, weight addresses, E, I, Is)``."""
     num = experts[0].shape[0]
     fmt, group, inner, ptrs = _moe_weights(experts, (num,), hidden, dev)
     if shared is None:
-        return fmt, group, ptrs + (None,) * 6, num, inner, 0
+        return fmt, group, ptrs + _NO_SHARED, num, inner, 0
     sfmt, sgroup, shared_inner, more = _moe_weights(shared, (), hidden, dev)
-    if sfmt != fmt or sgroup != group:
+    if (sfmt != fmt or sgroup != group or (shared[4] is None) != (experts[4] is None)
+            or (shared[5] is None) != (experts[5] is None)):
         _refuse("the shared expert must have the experts' format")
     return fmt, group, ptrs + more, num, inner, shared_inner
 
@@ -782,15 +804,18 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
     leaves out come out as 0 and choose nothing.  The gated product is rounded
     to bf16 once, its weight included; sums are fp32."""
     dev, t, hidden, stride, at = _moe_rows(x, token_mask, ids, weights)
-    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, dev, hidden, experts, shared)
+    fmt, group, ptrs, num, inner, shared_inner = _moe_args(hidden, dev, experts, shared)
     if (ids.dtype is not _I32 or ids.dim() != 2 or ids.shape[0] != t or not ids.is_contiguous()
             or weights.dtype is not _FP32 or weights.shape != ids.shape or not weights.is_contiguous()):
         _refuse(f"ids must be contiguous int32 [{t}, top_k] and weights fp32 alike")
     top_k = ids.shape[1]
-    out = _rows_out(x, dev, t, hidden, out)
+    if out is None:
+        out, out_stride = x.new_empty(t, hidden), hidden
+    else:
+        out_stride = _rows_out(x, dev, t, hidden, out)
     nbytes = lib().hca_moe_workspace_bytes(t, num, top_k, hidden, inner, shared_inner)
     ws = torch.empty(nbytes, dtype=_U8, device=x.device)
-    call("hca_moe_experts", out.data_ptr(), out.stride(0), at, stride, ids.data_ptr(), weights.data_ptr(), _p(token_mask), fmt,
+    call("hca_moe_experts", out.data_ptr(), out_stride, at, stride, ids.data_ptr(), weights.data_ptr(), _p(token_mask), fmt,
          group, *ptrs, t, num, hidden, inner, shared_inner, top_k, ws.data_ptr(), nbytes, _stream(dev))
     return out
 
@@ -804,14 +829,17 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts: MoEWeights
     ``[T, H]``.  Its scratch comes from the caching allocator on the current
     stream, so calls on several streams do not meet."""
     dev, t, hidden, stride, at = _moe_rows(x, token_mask, router_weight, router_bias)
-    fmt, group, ptrs, num, inner, shared_inner = _moe_args(x, dev, hidden, experts, shared)
+    fmt, group, ptrs, num, inner, shared_inner = _moe_args(hidden, dev, experts, shared)
     rows, wr, fp32, bias, sigmoid = _router_args(hidden, router_weight, router_bias, top_k, score)
     if rows != num:
         _refuse(f"router_weight must have the {num} experts' rows")
-    out = _rows_out(x, dev, t, hidden, out)
+    if out is None:
+        out, out_stride = x.new_empty(t, hidden), hidden
+    else:
+        out_stride = _rows_out(x, dev, t, hidden, out)
     nbytes = lib().hca_moe_workspace_bytes(t, num, top_k, hidden, inner, shared_inner)
     ws = x.new_empty((nbytes + 1) // 2)
-    call("hca_moe_decode", out.data_ptr(), out.stride(0), at, stride, wr, fp32, bias, sigmoid, renormalize, routed_scale,
+    call("hca_moe_decode", out.data_ptr(), out_stride, at, stride, wr, fp32, bias, sigmoid, renormalize, routed_scale,
          _p(token_mask), fmt, group, *ptrs, t, num, hidden, inner, shared_inner, top_k, ws.data_ptr(), nbytes, _stream(dev))
     return out
 
@@ -848,8 +876,8 @@ def apply_logit_penalties(logits: torch.Tensor, token_ids: torch.Tensor | None =
         _refuse("logits must be [rows, V]")
     rows, vocab = logits.shape
     logits_stride, inner = logits.stride()
-    if vocab == 0 or (vocab > 1 and inner != 1):
-        _refuse("logits must be [rows, V] with contiguous rows")
+    if vocab == 0 or (vocab > 1 and inner != 1) or (rows > 1 and logits_stride < vocab):
+        _refuse("logits must be [rows, V] with contiguous rows that do not overlap")
     reqs = rows
     for t in (token_ids, repetition, frequency, presence, bias_ids):
         if t is not None:
