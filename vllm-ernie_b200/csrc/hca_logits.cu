@@ -84,8 +84,15 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
     reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   if (threadIdx.x == 0) next_span = 0;
   pdl_wait_and_release();
+  // what the row needs, in two rounds of loads
   const int64_t req = a.req_index == nullptr ? row : a.req_index[row];
+  const bool history = a.token_ids != nullptr;
+  const int seq_len = history ? max(min(a.seq_lens[row], a.token_width), 0) : 0;
+  const int prompt_len = history ? max(min(a.prompt_lens[row], seq_len), 0) : 0;
   if (req < 0 || req >= a.num_reqs) return;  // the whole CTA
+  const float rep = a.repetition == nullptr ? 1.0f : a.repetition[req];
+  const float freq = a.frequency == nullptr ? 0.0f : a.frequency[req];
+  const float pres = a.presence == nullptr ? 0.0f : a.presence[req];
   T* logits = static_cast<T*>(a.logits) + row * a.stride;
   __syncthreads();
 
@@ -96,10 +103,8 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
     return ((static_cast<uint32_t>(v) ^ owner) & owner_mask) == 0 && static_cast<uint32_t>(v) < static_cast<uint32_t>(a.vocab);
   };
   auto place = [&](int32_t v) { return (v >> shift) * 32 + (v & 31); };
-  if (a.token_ids != nullptr) {
+  if (history) {
     const int32_t* tokens = a.token_ids + req * a.token_stride;
-    const int seq_len = max(min(a.seq_lens[row], a.token_width), 0);
-    const int prompt_len = max(min(a.prompt_lens[row], seq_len), 0);
     auto see = [&](int32_t v, bool answer) {
       if (!mine(v)) return;
       const int at = place(v);
@@ -117,10 +122,11 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
     for (int i = threadIdx.x; i < quads; i += kThreads) {
       const int4 v = body[i];
       const int at = head + 4 * i;
-      see(v.x, at >= prompt_len);
-      see(v.y, at + 1 >= prompt_len);
-      see(v.z, at + 2 >= prompt_len);
-      see(v.w, at + 3 >= prompt_len);
+      if (at >= prompt_len) {  // the same for almost every warp
+        see(v.x, true), see(v.y, true), see(v.z, true), see(v.w, true);
+      } else {
+        see(v.x, false), see(v.y, at + 1 >= prompt_len), see(v.z, at + 2 >= prompt_len), see(v.w, at + 3 >= prompt_len);
+      }
     }
     if (static_cast<int>(threadIdx.x) < seq_len - done)
       see(tokens[done + threadIdx.x], done + static_cast<int>(threadIdx.x) >= prompt_len);
@@ -132,9 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
   }
   __syncthreads();
 
-  const float rep = a.repetition == nullptr ? 1.0f : a.repetition[req], inverse = 1.0f / rep;
-  const float freq = a.frequency == nullptr ? 0.0f : a.frequency[req];
-  const float pres = a.presence == nullptr ? 0.0f : a.presence[req];
+  const float inverse = 1.0f / rep;
   const int32_t* allowed = a.allowed == nullptr ? nullptr : a.allowed + row * a.allowed_stride;
   auto penalise = [&](float x, uint32_t n, bool seen) {
     if (seen) x = x * (x > 0.0f ? inverse : rep);
