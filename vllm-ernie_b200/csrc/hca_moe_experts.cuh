@@ -432,14 +432,18 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr;
   auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
   // Warps to a tile: the number that makes the longest warp's work shortest (if
-  // every pair chose another expert), a tile's end costing about what a quad of
-  // units does.
+  // every pair chose another expert).  Runs begin and end inside an expert, so a
+  // round more than the average has to be counted; a tile's end costs half of
+  // what a quad of units does, and more the more warps meet there.  (e4m3, rows
+  // of 4096, 56 tiles a CTA: 122 us with one warp, 114 with two, 113 with four,
+  // 115 with eight; 4-bit, 112 tiles: 192, 188, 198, 240.)
   auto warps = [&](int64_t tiles, int64_t shared_tiles, int k, int least_k) {
     const int64_t n = std::min(p.routing.experts, p.tokens * p.routing.top_k) * tiles + shared_tiles;
     int best = 0;
-    int64_t least = INT64_MAX;
+    double least = INFINITY;
     for (int gw = 1; gw <= kWarps && 4 * gw <= W::units(least_k); gw *= 2) {
-      const int64_t cost = cdiv(cdiv(n, sms), kWarps / gw) * static_cast<int64_t>(cdiv(W::units(k), 4 * gw) + 1);
+      const double rounds = static_cast<double>(n) * gw / (kWarps * sms) + 1, quads = W::units(k) / (4.0 * gw);
+      const double cost = rounds * (quads + 0.5 + gw / 64.0);
       if (cost < least && columns + scales(k, gw) <= kSmem) least = cost, best = gw;
     }
     return best;
