@@ -9,7 +9,7 @@
 // few experts and lays out their columns in shared memory once.  The second
 // product leaves each (token, slot) pair's share of y in 32 bits, and the last
 // step adds a token's shares in the order of its slots: no atomics, and a
-// token's result does not depend on what else is in the batch.  h is rounded
+// token's result depends on how many others are in the batch, not on which.  h is rounded
 // to bf16 once, its weight included.
 //
 // One launch with two grid barriers, since each of the steps is short at one
@@ -29,6 +29,7 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 // shared memory of a CTA for columns and tile sums, beside the plan
 constexpr int64_t kSmem = 208 * 1024;
+static_assert(kWarps * 64 > kMoeExperts, "the plan's lanes hold two experts each");
 
 // Who computes what, made by every CTA from the ids (at most 1024 of them) in
 // shared memory.  A pair is t * top_k + j; the shared expert's are tokens *
@@ -47,6 +48,7 @@ struct Plan {
   float weight[kMoePairs];
   uint64_t who[kMoeExperts + 1];  // expert -> its tokens
   int16_t list[kMoeExperts + 1];  // expert -> first pair
+  int sums[kWarps];               // of 64 experts: pairs, and entries from bit 16 on
 };
 
 template <int kColumns>
@@ -96,30 +98,40 @@ __device__ __forceinline__ void build_plan(Plan<kColumns>& pl, const MoePass& p)
   for (int i = threadIdx.x; i < routed; i += kThreads)
     if (pl.id[i] >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&pl.who[pl.id[i]]), 1ull << token(i));
   __syncthreads();
-  if (threadIdx.x < 32) {
-    int entries = 0, pairs = 0;
-#pragma unroll 1
-    for (int e0 = 0; e0 <= experts; e0 += 32) {
-      const int e = e0 + lane;
-      const int c = e <= experts ? __popcll(pl.who[e]) : 0, pieces = (c + kColumns - 1) / kColumns;
-      int before = c | pieces << 16;  // inclusive sums of both
+  {
+    // pairs and entries before each expert, two experts a lane
+    const int warp = threadIdx.x >> 5, e0 = warp * 64 + 2 * lane;
+    auto pieces = [](int c) { return (c + kColumns - 1) / kColumns; };
+    int c[2], own = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-      }
-      const int first = pairs + (before & 0xffff) - c, at = entries + (before >> 16) - pieces;
-      if (c > 0) pl.list[e] = static_cast<int16_t>(first);
-#pragma unroll 1
-      for (int i = 0; i < pieces; ++i) {
-        pl.expert[at + i] = static_cast<int16_t>(e);
-        pl.start[at + i] = static_cast<int16_t>(first + i * kColumns);
-      }
-      if (e == experts) pl.routed = at;
-      const int all = __shfl_sync(0xffffffffu, before, 31);
-      pairs += all & 0xffff, entries += all >> 16;
+    for (int i = 0; i < 2; ++i) {
+      c[i] = e0 + i <= experts ? __popcll(pl.who[e0 + i]) : 0;
+      own += c[i] | pieces(c[i]) << 16;
     }
-    if (lane == 0) pl.entries = entries, pl.start[entries] = static_cast<int16_t>(pairs);
+    int at = own;  // inclusive sums of both
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += v;
+    }
+    if (lane == 31) pl.sums[warp] = at;
+    __syncthreads();
+    const int other = lane < kWarps ? pl.sums[lane] : 0;
+    at += static_cast<int>(__reduce_add_sync(0xffffffffu, lane < warp ? other : 0)) - own;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int e = e0 + i, first = at & 0xffff, entry = at >> 16;
+      if (c[i] > 0) pl.list[e] = static_cast<int16_t>(first);
+#pragma unroll 1
+      for (int j = 0; j < pieces(c[i]); ++j) {
+        pl.expert[entry + j] = static_cast<int16_t>(e);
+        pl.start[entry + j] = static_cast<int16_t>(first + j * kColumns);
+      }
+      if (e == experts) pl.routed = entry;
+      at += c[i] | pieces(c[i]) << 16;
+    }
+    const int all = static_cast<int>(__reduce_add_sync(0xffffffffu, other));
+    if (threadIdx.x == 0) pl.entries = all >> 16, pl.start[all >> 16] = static_cast<int16_t>(all & 0xffff);
   }
   __syncthreads();
 #pragma unroll 1
