@@ -29,6 +29,7 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 // shared memory of a CTA for columns and tile sums, beside the plan
 constexpr int64_t kSmem = 208 * 1024;
+constexpr int64_t kPrefetch = 256 * 1024;  // weights of a CTA on their way into L2 at the grid barrier
 static_assert(kWarps * 64 > kMoeExperts, "the plan's lanes hold two experts each");
 
 // Who computes what, made by every CTA from the ids (at most 1024 of them) in
@@ -317,6 +318,16 @@ struct Product {
     return true;
   }
 
+  // The segment's first weights into L2, by one thread.
+  __device__ __forceinline__ void prefetch() const {
+    const int tile = first.tile - g.id;  // thread 0's group
+    int64_t e;
+    const MoeMatrix& m = matrix(first, e);
+    const int64_t row = W::row_bytes(k_of(first_entry));
+    const int n = min(to - from, tiles - tile);
+    if (n > 0) prefetch_weights(m.data + (e * p.hidden + tile * 16) * row, min(n * 16 * row, kPrefetch));
+  }
+
   // Lays out the segment's columns and consumes its tiles.  Both ends are
   // block barriers for the columns.
   template <typename Stream>
@@ -398,6 +409,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   {
     Product<F, NB, kWidth, false> down(p, w, pl, smem, room, scales, shape.down_warps, false);
     bool more = down.start(stream);
+    // bf16 weights come slower than they are used, so they go on coming while
+    // the CTAs meet (38.8 -> 37.9 us at one token; 4-bit and e4m3 lost 0.5 %)
+    if (F == kWBf16 && more && threadIdx.x == 0) down.prefetch();
     if (!grid_wait(p.barrier, 1, p.error)) {
       asm volatile("cp.async.wait_all;\n" ::: "memory");
       return;

@@ -466,6 +466,11 @@ __device__ __forceinline__ void load_weights(uint32_t (&w)[4], const uint8_t* p)
                : "l"(p));
 }
 
+// Brings the first `bytes` (a multiple of 16) from p on into L2.
+__device__ __forceinline__ void prefetch_weights(const uint8_t* p, int64_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(p), "r"(static_cast<uint32_t>(bytes)) : "memory");
+}
+
 // The lane's two rows of a tile (fragment rows lane / 4 and lane / 4 + 8), from
 // 16 (lane % 4) bytes on.
 struct TileRows {

@@ -31,6 +31,7 @@ struct W4Args {
   const uint8_t* zeros;
   int tokens, n, k;
   int group_warps;  // warps that share a tile
+  int ahead;        // whether a group's first tile is fetched into L2 before all else
 };
 
 // The tiles of a group of warps: first, first + stride, ...
@@ -76,6 +77,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   const int columns = min(X::kColumns, a.tokens - t0), live = (columns + kWidth - 1) / kWidth;
   W4Tiles<F, T> src{a, static_cast<int>(blockIdx.x + g.id * gridDim.x), static_cast<int>(gridDim.x) * per_cta, a.k / W::kGroupK};
 
+  if (g.thread() == 0 && a.ahead && src.first < tiles)
+    prefetch_weights(a.q + src.first * 16ll * W::row_bytes(a.k), min(16, a.n - src.first * 16) * W::row_bytes(a.k));
   pdl_wait_and_release();
   TileStream<F, T, WTraits<F>::step(NB)> stream;
   stream.start(a.k, g, src.first < tiles ? (tiles - src.first + src.stride - 1) / src.stride : 0,
@@ -172,6 +175,9 @@ bool launch(W4Args a, cudaStream_t s, int& rc) {
     if (cost < best && columns + scales(gw) <= kSmem) best = cost, a.group_warps = gw;
   }
   if (a.group_warps == 0) return false;
+  // Weights that last for a round or two start before the kernel before this
+  // one has ended (11.6 -> 10.8 us for 8192 x 4096 and 16 rows, weights not in L2).
+  a.ahead = tiles <= 2 * sms * (kWarps / a.group_warps);
   const int64_t smem = columns + scales(a.group_warps);
   static bool done[kMaxDevices] = {};
   rc = set_func_attr_once(w4_linear_kernel<F, T, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
@@ -219,7 +225,7 @@ extern "C" int hca_w4_linear(void* out, int64_t out_stride, const void* x, int64
   HCA_CHECK_ARG(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0 &&
                 reinterpret_cast<uintptr_t>(zeros) % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 2 == 0);
   HCA_CHECK_ARG(num_tokens <= 65535 && n <= INT32_MAX - 16);  // grid columns hold at least one row of x
-  W4Args a{out, out_stride, x, x_stride, q, scales, zeros, num_tokens, n, k, 1};
+  W4Args a{out, out_stride, x, x_stride, q, scales, zeros, num_tokens, n, k, 1, 0};
   cudaStream_t s = as_stream(stream);
   return is_fp16 ? by_group<__half>(group_size, a, s) : by_group<__nv_bfloat16>(group_size, a, s);
 }
