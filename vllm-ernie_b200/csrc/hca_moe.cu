@@ -8,8 +8,9 @@
 // so they are spread over the whole GPU: a CTA computes two to four experts
 // for up to eight tokens, its warps splitting hidden.  Products and sums are
 // 32-bit multiply-adds: a bf16 tensor product would make near-ties of a 32-bit
-// router fall differently.  The choice itself is one warp's work a token, and
-// every CTA of the expert kernel makes it for itself.
+// router fall differently.  The choice itself is one warp's work a token, and up
+// to 16 tokens every CTA of the expert kernel makes it for itself.  About 3 us
+// for 64 experts of 4096 and one token, most of it launch and one round of loads.
 #include "hca_moe.cuh"
 #include "hca_stream.cuh"
 

@@ -20,25 +20,29 @@
 // quad on its way in registers while one is consumed, across the ends of
 // tiles; rows are padded to whole quads with activations that are zero, so the
 // loop over quads has no branches.  (Rings in shared memory, filled by TMA
-// boxes or asynchronous copies, came to 3.7 TB/s where this comes to 5: each
-// unit then starts with a wait and a read that nothing overlaps.)  A product may only sum
-// over one group of codes; with groups of 64 or 32 the four lanes exchange
-// words first.  Sums are held in 32 bits; group and block scales multiply the
-// 32-bit sums of their own groups.  The 4-bit scales and zero points of a
-// warp's share of a tile come into shared memory a tile ahead, in runs along the
-// rows: loaded unit by unit they cost L1 more cycles than the codes.
+// boxes or asynchronous copies, came to 3.7 TB/s where this comes to 5.2, with
+// 4-bit weights [129281, 4096] and 8 rows: each unit then starts with a wait and
+// a read that nothing overlaps.)  What is on its way needs lines of L1, so a CTA
+// takes no more shared memory than it must: with 64 KB more for further columns
+// the expert layer's time rose from 192 to 268 us.
+//
+// A product may only sum over one group of codes; with groups of 64 or 32 the
+// four lanes exchange words first.  Sums are held in 32 bits; group and block
+// scales multiply the 32-bit sums of their own groups.  The 4-bit scales and zero
+// points of a warp's share of a tile come into shared memory a tile ahead, in
+// runs along the rows: loaded unit by unit they cost L1 more cycles than the
+// codes.
 //
 // No code is converted.  The smallest floats of a 16-bit type are evenly
 // spaced: bits 0..7 of a bf16 (0..10 of an fp16) with nothing above them are
 // the number times 2^-133 (2^-24), across the end of the subnormals.  So a
 // word of 4-bit codes, masked, is two codes as exact floats, and those four
 // bits higher are 16 times theirs: five bit operations for eight codes.  e4m3
-// moved into the low
-// exponent and high mantissa bits of a bf16 is its value times 2^-120, the
-// subnormals with it.  bf16 activations are scaled by 2^80 when they are laid
-// out, so that the products keep clear of both ends of the 32-bit range for
-// |x| from 2^-73 to 2^47, and the powers of two leave with the finished sum.
-// An e4m3 NaN would count as 480; an infinite x makes its row NaN.
+// moved into the low exponent and high mantissa bits of a bf16 is its value
+// times 2^-120, the subnormals with it.  bf16 activations are scaled by 2^80
+// when they are laid out, so that the products keep clear of both ends of the
+// 32-bit range for |x| from 2^-73 to 2^47, and the powers of two leave with the
+// finished sum.  An e4m3 NaN counts as 480; an infinite x makes its row NaN.
 //
 // Zero points come off the group's sum: s (sum q x - z sum x), with sum x
 // known once per column and group, where taking z from every code costs half

@@ -615,18 +615,33 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
     in fp32, one rounding to x's type.  ``out`` must not overlap ``x``.  Right
     for any T, made for up to 16 rows (each 16 more read the weights again; a
     prompt's thousands belong on a dense product)."""
-    dev = _device_of(x, qweight, scales, zeros)
+    # in line, as the shortest of these calls take the GPU 4 us
+    dev = x.get_device()
+    if not -1 < dev == qweight.get_device() == scales.get_device() == torch._C._cuda_getDevice():
+        _refuse("libhca_b200 ops take CUDA tensors of the current device")
     dtype = x.dtype
     if dtype is not _BF16 and dtype is not _FP16:
         _refuse(f"x must be bf16 or fp16, got {dtype}")
-    t, k, stride, at = _check_rows(x)
     try:
-        n, _ = qweight.shape
+        (t, k), (n, half), (rows, groups) = x.shape, qweight.shape, scales.shape
     except ValueError:
-        _refuse("qweight must be [N, K / 2]")
-    if n == 0:
-        _refuse("qweight has no rows")
-    group = _check_w4(qweight, scales, zeros, (), n, k, dtype)
+        _refuse("x must be [T, K], qweight [N, K / 2] and scales [N, K / g]")
+    stride, inner = x.stride()
+    at = x.data_ptr()
+    if inner != 1 or (stride % 8 and t > 1) or at % 16:
+        _refuse("x must have contiguous rows that start on 16 bytes")
+    if qweight.dtype is not _U8 or n == 0 or 2 * half != k or not qweight.is_contiguous():
+        _refuse(f"4-bit codes must be contiguous uint8 {[n, k // 2]}")
+    if scales.dtype is not dtype or rows != n or groups == 0 or k % groups or not scales.is_contiguous():
+        _refuse(f"scales must be contiguous {dtype} [{n}, K / g]")
+    group = k // groups
+    if group not in W4_GROUPS:
+        _refuse(f"the group size must be one of {W4_GROUPS}, got {group}")
+    if zeros is not None and (zeros.get_device() != dev or zeros.dtype is not _U8 or zeros.shape != (n, groups)
+                              or not zeros.is_contiguous()):
+        _refuse("zero points must be contiguous uint8 of the scales' shape")
+    if t < 2:
+        stride = k
     if out is None:
         out, out_stride = x.new_empty(t, n), n
     else:
