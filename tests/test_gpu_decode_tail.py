@@ -769,6 +769,20 @@ def test_moe_experts_long_rows(tokens, hidden, inner, shared, kind):
     _within(got, ref, _moe_bound(ref, size, hidden + 2 * inner + shared))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "w4-32z"])
+@pytest.mark.parametrize("hidden,inner,shared", [(512, 64, 16384), (16384, 16384, 32), (64, 32, 8192)])
+def test_moe_experts_of_very_different_lengths(hidden, inner, shared, kind):
+    gen = _gen(hidden + shared)
+    x = torch.randn((3, hidden), generator=gen, device=DEV).to(torch.bfloat16)
+    stack, w13, w2 = _stack(kind, (2,), hidden, inner, gen)
+    one, a, b = _stack(kind, (), hidden, shared, gen)
+    ids = torch.tensor([[0], [1], [0]], device=DEV, dtype=torch.int32)
+    weights = torch.rand((3, 1), generator=gen, device=DEV)
+    got = _ops().moe_experts(x, ids, weights, stack, shared=one)
+    ref, size = _experts_ref(x, ids, weights, w13, w2, shared=(a, b))
+    _within(got, ref, _moe_bound(ref, size, hidden + inner + shared))
+
+
 @pytest.mark.parametrize("tokens", [1, 3, 16, 17, 64])
 @pytest.mark.parametrize("experts,k", [(129, 6), (512, 16)])
 def test_moe_decode_of_many_experts_is_route_then_experts(experts, k, tokens):

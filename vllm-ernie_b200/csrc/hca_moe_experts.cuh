@@ -475,7 +475,8 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
     const int64_t n = std::min(p.routing.experts, p.tokens * p.routing.top_k) * tiles + shared_tiles;
     int best = 0;
     double least = INFINITY;
-    for (int gw = 1; gw <= kWarps && 4 * gw <= W::units(least_k); gw *= 2) {
+    // (no more than the shorter rows have quads, unless scales need the room)
+    for (int gw = 1; gw <= kWarps && (4 * gw <= W::units(least_k) || best == 0); gw *= 2) {
       const double rounds = static_cast<double>(n) * gw / (kWarps * sms) + 1, quads = W::units(k) / (4.0 * gw);
       const double cost = rounds * (quads + 0.5 + gw / 64.0);
       if (cost < least && columns + scales(k, gw) <= kSmem) least = cost, best = gw;
