@@ -882,14 +882,16 @@ def apply_logit_penalties(logits: torch.Tensor, token_ids: torch.Tensor | None =
     and ``bias_values`` fp32 ``[R, M]`` (of an id listed twice the later
     counts); ids outside ``[0, V)``, like -1, are skipped.  ``allowed_bitmask``
     int32 ``[rows, ceil(V / 32)]``, bit ``v % 32`` of word ``v // 32``."""
-    dev = _device_of(logits, token_ids, prompt_lens, seq_lens, repetition, frequency, presence, bias_ids, bias_values,
-                     allowed_bitmask, req_index)
+    dev = logits.get_device()
+    if not -1 < dev == torch._C._cuda_getDevice():
+        _refuse("libhca_b200 ops take CUDA tensors of the current device")
     kind = _LOGIT_TYPES.get(logits.dtype, -1)
     if kind < 0:
         _refuse(f"logits must be fp32, bf16 or fp16, got {logits.dtype}")
-    if logits.dim() != 2:
+    try:
+        rows, vocab = logits.shape
+    except ValueError:
         _refuse("logits must be [rows, V]")
-    rows, vocab = logits.shape
     logits_stride, inner = logits.stride()
     if vocab == 0 or (vocab > 1 and inner != 1) or (rows > 1 and logits_stride < vocab):
         _refuse("logits must be [rows, V] with contiguous rows that do not overlap")
@@ -898,42 +900,52 @@ def apply_logit_penalties(logits: torch.Tensor, token_ids: torch.Tensor | None =
         if t is not None:
             reqs = t.shape[0]
             break
-    for t in (repetition, frequency, presence):
-        if t is not None and (t.dtype is not _FP32 or t.shape != (reqs,) or not t.is_contiguous()):
-            _refuse(f"penalties must be contiguous fp32 [{reqs}]")
+    at = [0, 0, 0]  # addresses of the penalties
+    for i, t in enumerate((repetition, frequency, presence)):
+        if t is not None:
+            if t.dtype is not _FP32 or t.shape != (reqs,) or not t.is_contiguous() or t.get_device() != dev:
+                _refuse(f"penalties must be contiguous fp32 [{reqs}] on the logits' device")
+            at[i] = t.data_ptr()
+    index = 0
     if req_index is None:
         if reqs != rows:
             _refuse(f"{reqs} requests for {rows} rows need req_index")
-    elif req_index.dtype is not _I32 or req_index.shape != (rows,) or not req_index.is_contiguous():
-        _refuse(f"req_index must be contiguous int32 [{rows}]")
-    width = stride = 0
+    else:
+        if (req_index.dtype is not _I32 or req_index.shape != (rows,) or not req_index.is_contiguous()
+                or req_index.get_device() != dev):
+            _refuse(f"req_index must be contiguous int32 [{rows}] on the logits' device")
+        index = req_index.data_ptr()
+    width = stride = tokens = prompts = lens = 0
     if token_ids is not None:
-        if token_ids.dtype is not _I32 or token_ids.dim() != 2 or token_ids.shape[0] != reqs:
-            _refuse(f"token_ids must be int32 [{reqs}, L]")
+        if token_ids.dtype is not _I32 or token_ids.dim() != 2 or token_ids.shape[0] != reqs or token_ids.get_device() != dev:
+            _refuse(f"token_ids must be int32 [{reqs}, L] on the logits' device")
         width = token_ids.shape[1]
         stride, inner = token_ids.stride()
         if width > 1 and inner != 1:
             _refuse("token_ids must have contiguous rows")
         for t in (prompt_lens, seq_lens):
-            if t is None or t.dtype is not _I32 or t.shape != (rows,) or not t.is_contiguous():
-                _refuse(f"prompt_lens and seq_lens must be contiguous int32 [{rows}]")
-    bias_width = 0
-    if (bias_ids is None) != (bias_values is None):
-        _refuse("bias_ids and bias_values come together")
-    if bias_ids is not None:
+            if t is None or t.dtype is not _I32 or t.shape != (rows,) or not t.is_contiguous() or t.get_device() != dev:
+                _refuse(f"prompt_lens and seq_lens must be contiguous int32 [{rows}] on the logits' device")
+        tokens, prompts, lens = token_ids.data_ptr(), prompt_lens.data_ptr(), seq_lens.data_ptr()
+    bias_width = biases = values = 0
+    if bias_ids is not None or bias_values is not None:
+        if bias_ids is None or bias_values is None:
+            _refuse("bias_ids and bias_values come together")
         if (bias_ids.dtype is not _I32 or bias_ids.dim() != 2 or bias_ids.shape[0] != reqs or not bias_ids.is_contiguous()
-                or bias_values.dtype is not _FP32 or bias_values.shape != bias_ids.shape or not bias_values.is_contiguous()):
-            _refuse(f"bias_ids must be contiguous int32 [{reqs}, M] and bias_values fp32 alike")
-        bias_width = bias_ids.shape[1]
-    allowed_stride = 0
+                or bias_values.dtype is not _FP32 or bias_values.shape != bias_ids.shape or not bias_values.is_contiguous()
+                or not bias_ids.get_device() == bias_values.get_device() == dev):
+            _refuse(f"bias_ids must be contiguous int32 [{reqs}, M] and bias_values fp32 alike, on the logits' device")
+        bias_width, biases, values = bias_ids.shape[1], bias_ids.data_ptr(), bias_values.data_ptr()
+    allowed_stride = allowed = 0
     if allowed_bitmask is not None:
         words = (vocab + 31) // 32
-        if allowed_bitmask.dtype is not _I32 or allowed_bitmask.shape != (rows, words):
-            _refuse(f"allowed_bitmask must be int32 [{rows}, {words}]")
+        if (allowed_bitmask.dtype is not _I32 or allowed_bitmask.shape != (rows, words)
+                or allowed_bitmask.get_device() != dev):
+            _refuse(f"allowed_bitmask must be int32 [{rows}, {words}] on the logits' device")
         allowed_stride, inner = allowed_bitmask.stride()
         if words > 1 and inner != 1:
             _refuse("allowed_bitmask must have contiguous rows")
-    call("hca_logit_penalties", logits.data_ptr(), logits_stride, kind, _p(req_index), reqs, _p(token_ids), stride, width,
-         _p(prompt_lens), _p(seq_lens), _p(repetition), _p(frequency), _p(presence), _p(bias_ids), _p(bias_values),
-         bias_width, bias_width, _p(allowed_bitmask), allowed_stride, rows, vocab, _stream(dev))
+        allowed = allowed_bitmask.data_ptr()
+    call("hca_logit_penalties", logits.data_ptr(), logits_stride, kind, index, reqs, tokens, stride, width, prompts, lens,
+         at[0], at[1], at[2], biases, values, bias_width, bias_width, allowed, allowed_stride, rows, vocab, _stream(dev))
     return logits
