@@ -874,3 +874,15 @@ def test_logit_penalties_refuse_rows_on_top_of_each_other():
 
 def test_no_wait_gave_up():
     assert _ops().device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,length,bias,mask", [
+    (200, 5003, 300, 6, True),     # more rows than SMs, small tables
+    (150, 32000, 40, 0, False),
+    (300, 17, 0, 2, True),
+    (2, 3000, 70000, 4, True),     # counts past 16 bits
+    (170, 900, 66000, 0, False),
+])
+def test_logit_penalties_many_rows_and_long_histories(rows, vocab, length, bias, mask, dtype):
+    test_logit_penalties(rows, vocab, length, bias, mask, dtype)

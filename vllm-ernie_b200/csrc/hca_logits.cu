@@ -27,9 +27,8 @@
 namespace hca {
 namespace {
 
-constexpr int kThreads = 1024;
 constexpr int kAhead = 2;  // logits of a lane under way
-constexpr int kSmem = 224 * 1024;
+constexpr int kSmem = 224 * 1024;  // of an SM, for one CTA of 1024 threads or two of 512
 
 __device__ __forceinline__ float load_logit(const float* p) { return *p; }
 __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -64,14 +63,14 @@ template <typename Count>
 struct Tables {
   static constexpr int kEntry = static_cast<int>(sizeof(Count));
   static constexpr int kSpan = 16;  // tokens of a lane at a time
-  static constexpr int kListBytes = kThreads * kSpan * 2;
+  static constexpr int kListBytes = kSpan * 2;  // of a thread
   // chunks, rounded up so that every lane's span exists
   static __host__ __device__ int64_t padded(int64_t chunks) { return (chunks + 15) / 16 * 16; }
   static __host__ __device__ int64_t bytes(int64_t chunks) { return padded(chunks) * (8 + 32 * kEntry); }
 };
 
-template <typename T, typename Count>
-__global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a) {
+template <typename T, typename Count, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) logit_penalty_kernel(LogitArgs a) {
   using Tab = Tables<Count>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int next_span;
@@ -234,30 +233,37 @@ __global__ void __launch_bounds__(kThreads, 1) logit_penalty_kernel(LogitArgs a)
   }
 }
 
-template <typename T, typename Count>
+template <typename T, typename Count, int kThreads>
 int launch(LogitArgs a, int rows, cudaStream_t s) {
   using Tab = Tables<Count>;
+  constexpr int kMost = kSmem / (1024 / kThreads);
   const int64_t chunks = (static_cast<int64_t>(a.vocab) + 31) / 32, sms = device_sm_count();
-  auto bytes = [&](int log2) { return Tab::bytes((chunks + (1 << log2) - 1) >> log2) + Tab::kListBytes; };
+  auto bytes = [&](int log2) { return Tab::bytes((chunks + (1 << log2) - 1) >> log2) + Tab::kListBytes * kThreads; };
   // Slices of a row: as few as shared memory allows, since each reads the
   // history; while they leave half the SMs without work twice as many, down to
   // 64 chunks each.
   a.slices_log2 = 0;
-  while (bytes(a.slices_log2) > kSmem ||
+  while (bytes(a.slices_log2) > kMost ||
          ((static_cast<int64_t>(rows) << (a.slices_log2 + 1)) <= sms && (chunks >> a.slices_log2) >= 128))
     ++a.slices_log2;
   if ((static_cast<int64_t>(rows) << a.slices_log2) > INT32_MAX) return HCA_E_INVALID;
+  // Two CTAs an SM where there are more rows than SMs and a row's tables take
+  // half of an SM's memory at most (256 rows of 32000: 9.3 us for 12.6); longer
+  // rows would need twice the slices (192 of 151937: 68 us for 57).
+  if constexpr (kThreads == 1024)
+    if (a.slices_log2 == 0 && rows > sms && Tab::bytes(chunks) + Tab::kListBytes * 512 <= kSmem / 2)
+      return launch<T, Count, 512>(a, rows, s);
   static bool done[kMaxDevices] = {};
-  if (set_func_attr_once(logit_penalty_kernel<T, Count>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done) !=
-      HCA_OK)
+  if (set_func_attr_once(logit_penalty_kernel<T, Count, kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost,
+                         done) != HCA_OK)
     return HCA_E_CUDA;
-  return launch_pdl(logit_penalty_kernel<T, Count>, dim3(static_cast<unsigned>(rows) << a.slices_log2), dim3(kThreads),
-                    static_cast<size_t>(bytes(a.slices_log2)), s, a);
+  return launch_pdl(logit_penalty_kernel<T, Count, kThreads>, dim3(static_cast<unsigned>(rows) << a.slices_log2),
+                    dim3(kThreads), static_cast<size_t>(bytes(a.slices_log2)), s, a);
 }
 
 template <typename T>
 int by_count(const LogitArgs& a, int rows, cudaStream_t s) {
-  return a.token_width <= 65535 ? launch<T, uint16_t>(a, rows, s) : launch<T, uint32_t>(a, rows, s);
+  return a.token_width <= 65535 ? launch<T, uint16_t, 1024>(a, rows, s) : launch<T, uint32_t, 1024>(a, rows, s);
 }
 
 }  // namespace
