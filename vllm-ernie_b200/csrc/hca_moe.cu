@@ -174,7 +174,7 @@ struct Scratch {
     const int64_t t = std::min(tokens, kMoeTokens);
     passes = cdiv(tokens, kMoeTokens);
     h = 0;
-    part = align_up(t * (static_cast<int64_t>(top_k) * inner + shared_inner) * 2);
+    part = align_up(t * (static_cast<int64_t>(top_k) * inner + shared_inner) * 4);  // h in two bf16 parts
     barriers = part + align_up(t * (top_k + 1) * hidden * 4);
     logits = barriers + align_up(4ll * passes);
     ids = logits + logit_bytes(tokens, experts);

@@ -33,7 +33,7 @@ struct MoePass {
   const float* logits;   // [tokens, experts], or null: ids and weights are given
   const int32_t* ids;    // [tokens, top_k], negative or >= experts: skipped
   const float* weights;  // [tokens, top_k]
-  __nv_bfloat16* h;      // [tokens * top_k, inner], then [tokens, shared_inner]
+  __nv_bfloat16* h;      // [tokens * top_k, 2, inner], then [tokens, 2, shared_inner]: rounded, and what that left
   float* part;           // [tokens * (top_k + 1), hidden]: a pair's share of y
   uint32_t* barrier;     // 0 before the launch
   int32_t* error;        // device error word

@@ -185,15 +185,16 @@ __device__ __forceinline__ bool grid_wait(uint32_t* barrier, uint32_t phase, int
 struct Shape {
   int up_warps, down_warps;  // warps that share a tile of either product
   int dense;                 // the first product's columns are the tokens, the same for every expert
+  int room;                  // bytes for columns
 };
 
 // One of the products over this CTA's run of (entry, tile) items.  kUp: h from
 // x (fragment rows 0..7 of a tile are gate rows, 8..15 the up rows of the same
 // inner columns, so a lane holds both factors); else part from h.
-template <int F, int NB, int kWidth, bool kUp>
+template <int F, int NB, int kWidth, int kParts, bool kUp>
 struct Product {
   using W = WTraits<F>;
-  using X = XTile<F, __nv_bfloat16, NB, kWidth>;
+  using X = XTile<F, __nv_bfloat16, NB, kWidth, kUp ? 1 : kParts>;
   using P = Plan<NB * kWidth>;
   const MoePass& p;
   const MoeWeights& w;
@@ -293,8 +294,8 @@ struct Product {
   __device__ __forceinline__ WScales here(int, int r) const { return scales_of(now, r); }
 
   __device__ __forceinline__ __nv_bfloat16* h_row(int pair) const {
-    return pair < pairs ? p.h + static_cast<int64_t>(pair) * p.inner
-                        : p.h + static_cast<int64_t>(pairs) * p.inner + static_cast<int64_t>(pair - pairs) * p.shared_inner;
+    return p.h + kParts * (pair < pairs ? static_cast<int64_t>(pair) * p.inner
+                                        : static_cast<int64_t>(pairs) * p.inner + static_cast<int64_t>(pair - pairs) * p.shared_inner);
   }
   __device__ __forceinline__ int token(int pair) const { return pair < pairs ? pair / p.routing.top_k : pair - pairs; }
 
@@ -383,7 +384,14 @@ struct Product {
         const float v = TileSums<NB>::sum(sums, g, c, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
         if (kUp) {
           const float up = TileSums<NB>::sum(sums, g, c + 8, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
-          h_row(pair)[now.tile * 8 + c] = __float2bfloat16_rn(__fdividef(v, 1.0f + __expf(-v)) * up * pl.weight[pair]);
+          const float h = __fdividef(v, 1.0f + __expf(-v)) * up * pl.weight[pair];
+          __nv_bfloat16* to = h_row(pair) + now.tile * 8 + c;
+          const __nv_bfloat16 first = __float2bfloat16_rn(h);
+          *to = first;
+          if (kParts == 2) {
+            const float rest = h - __bfloat162float(first);
+            to[now.entry >= pl.routed ? p.shared_inner : p.inner] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
+          }
         } else {
           p.part[static_cast<int64_t>(pair) * p.hidden + now.tile * 16 + c] = v;
         }
@@ -397,25 +405,24 @@ struct Product {
   }
 };
 
-template <int F, int NB, int kWidth>
+template <int F, int NB, int kWidth, int kParts>
 __global__ void __launch_bounds__(kThreads, 1)
     moe_layer_kernel(MoePass p, MoeWeights w, Shape shape) {
-  using X = XTile<F, __nv_bfloat16, NB, kWidth>;
   __shared__ Plan<NB * kWidth> pl;
   extern __shared__ __align__(16) uint8_t smem[];
   build_plan(pl, p);
   TileStream<F, __nv_bfloat16, WTraits<F>::step(NB)> stream;
-  const int room = static_cast<int>(X::bytes(WTraits<F>::units(max(p.hidden, max(p.inner, p.shared_inner)))));
+  const int room = shape.room;
   uint8_t* sums = smem + room;
   TileSums<NB> ts(sums);
   uint8_t* scales = sums + TileSums<NB>::bytes(kWarps);
   {
-    Product<F, NB, kWidth, true> up(p, w, pl, smem, room, scales, shape.up_warps, shape.dense);
+    Product<F, NB, kWidth, kParts, true> up(p, w, pl, smem, room, scales, shape.up_warps, shape.dense);
     while (up.start(stream)) up.run(stream, ts);
   }
   grid_arrive(p.barrier);
   {
-    Product<F, NB, kWidth, false> down(p, w, pl, smem, room, scales, shape.down_warps, false);
+    Product<F, NB, kWidth, kParts, false> down(p, w, pl, smem, room, scales, shape.down_warps, false);
     bool more = down.start(stream);
     // bf16 weights come slower than they are used, so they go on coming while
     // the CTAs meet (38.8 -> 37.9 us at one token; 4-bit and e4m3 lost 0.5 %)
@@ -452,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Launches with entries of NB blocks of kWidth columns if shared memory holds them.
-template <int F, int NB, int kWidth>
+template <int F, int NB, int kWidth, int kParts = 2>
 bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   using W = WTraits<F>;
   const int sms = device_sm_count();
@@ -461,8 +468,10 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   const int64_t units = std::max(static_cast<int64_t>(inner / 8) * W::units(p.hidden),
                                  static_cast<int64_t>(p.hidden / 16) * W::units(inner));
   if (units * p.tokens * (p.routing.top_k + 1) > UINT32_MAX) return false;
-  const int64_t columns = XTile<F, __nv_bfloat16, NB, kWidth>::bytes(W::units(std::max(p.hidden, inner))) +
-                          TileSums<NB>::bytes(kWarps);
+  Shape shape;
+  shape.room = static_cast<int>(std::max(XTile<F, __nv_bfloat16, NB, kWidth>::bytes(W::units(p.hidden)),
+                                         XTile<F, __nv_bfloat16, NB, kWidth, kParts>::bytes(W::units(inner))));
+  const int64_t columns = shape.room + TileSums<NB>::bytes(kWarps);
   const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr;
   auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
   // Warps to a tile: the number that makes the longest warp's work shortest (if
@@ -483,7 +492,6 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
     }
     return best;
   };
-  Shape shape;
   shape.up_warps = warps(p.inner / 8, p.shared_inner / 8, p.hidden, p.hidden);
   shape.down_warps = warps(p.hidden / 16, p.shared_inner > 0 ? p.hidden / 16 : 0, inner,
                            p.shared_inner > 0 ? std::min(p.inner, p.shared_inner) : p.inner);
@@ -492,7 +500,7 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   if (shape.up_warps == 0 || shape.down_warps == 0) return false;
   const int64_t smem = columns + std::max(scales(p.hidden, shape.up_warps), scales(inner, shape.down_warps));
   static bool done[kMaxDevices] = {};
-  rc = set_func_attr_once(moe_layer_kernel<F, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
+  rc = set_func_attr_once(moe_layer_kernel<F, NB, kWidth, kParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
   if (rc != HCA_OK) return true;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeCooperative;
@@ -504,7 +512,7 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  rc = cuda_status(cudaLaunchKernelEx(&cfg, moe_layer_kernel<F, NB, kWidth>, p, w, shape));
+  rc = cuda_status(cudaLaunchKernelEx(&cfg, moe_layer_kernel<F, NB, kWidth, kParts>, p, w, shape));
   return true;
 }
 
@@ -526,6 +534,8 @@ int moe_experts_pass(const MoePass& p, const MoeWeights& w, cudaStream_t s) {
   if (p.tokens > 4 && moe::launch<F, 1, 8>(p, w, s, rc)) return rc;
   if (p.tokens > 2 && moe::launch<F, 1, 4>(p, w, s, rc)) return rc;
   if (moe::launch<F, 1, 2>(p, w, s, rc)) return rc;
+  // rows of h too long for two parts: rounded to bf16 once
+  if (moe::launch<F, 1, 2, 1>(p, w, s, rc)) return rc;
   return HCA_E_UNSUPPORTED;
 }
 

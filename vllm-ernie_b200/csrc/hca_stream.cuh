@@ -169,8 +169,8 @@ template <int F>
 __device__ __forceinline__ int piece_swap(int u, int j) {
   return F == kWBf16 ? 4 * (u & 1) : F == kW4G128 ? 2 * j : 4 * (j & 1);
 }
-template <int F, int kWidth>
-__device__ __forceinline__ int piece_index(int k, int col) {
+template <int F, int kWidth, int kParts>
+__device__ __forceinline__ int piece_index(int k, int col, int part) {
   using W = WTraits<F>;
   const int u = k / W::kUnitK, r = k % W::kUnitK;
   int c, j;
@@ -179,7 +179,7 @@ __device__ __forceinline__ int piece_index(int k, int col) {
   else if constexpr (F == kW4G128) c = r / 32, j = r / 8 % 4;
   else if constexpr (F == kW4G64) c = r / 32 % 2 + r / 16 % 2 * 2, j = r / 64 * 2 + r / 8 % 2;
   else c = r / 8 % 4, j = r / 32;
-  return (u * W::kPieces + j) * kWidth * 4 + ((col * 4 + c) ^ piece_swap<F>(u, j));
+  return ((u * W::kPieces + j) * kParts + part) * kWidth * 4 + ((col * 4 + c) ^ piece_swap<F>(u, j));
 }
 
 // Eight consecutive activations in a piece's order, that in which weights come
@@ -290,15 +290,17 @@ struct ScaleTile {
 };
 
 // Activations of NB blocks of columns in shared memory, in piece order, with
-// their group sums.  A block has 8 columns, of which kWidth are stored.
-template <int F, typename T, int NB, int kWidth>
+// their group sums.  A block has 8 columns, of which kWidth are stored.  With
+// two parts an activation is the sum of two numbers, the second what rounding
+// the first left: a second product with the same weights adds it.
+template <int F, typename T, int NB, int kWidth, int kParts = 1>
 struct XTile {
   using W = WTraits<F>;
-  uint4* pieces;  // [NB][units][kPieces][kWidth][4]
+  uint4* pieces;  // [NB][units][kPieces][kParts][kWidth][4]
   float* sums;    // [NB][units][kSub][8], 4-bit only
   int units;
 
-  static constexpr int kUnitPieces = W::kPieces * kWidth * 4;
+  static constexpr int kUnitPieces = W::kPieces * kParts * kWidth * 4;
   static constexpr int kColumns = NB * kWidth;
   // Group sums of x by the tensor instructions once it is laid out, which costs
   // the same for one column as for eight, or by adding on the way: 16 rows of
@@ -314,37 +316,48 @@ struct XTile {
     sums = reinterpret_cast<float*>(smem + static_cast<int64_t>(NB) * units * kUnitPieces * 16);
   }
 
-  // All threads of the block; row(col) is column col's row of k values or
-  // null (zeros, as in the columns after `columns`).  Ends with a block barrier.
+  // All threads of the block; row(col) is column col's row of k values (and
+  // behind them the k second parts) or null (zeros, as in the columns after
+  // `columns`).  Ends with a block barrier.
   template <typename Row>
   __device__ __forceinline__ void stage(int k, int columns, int live, Row row) {
     const int padded = units * W::kUnitK;
     // several columns' loads under way at a time
-    constexpr int kAhead = kWidth;
+    constexpr int kAhead = kWidth * kParts > 8 ? 8 / kParts : kWidth;
 #pragma unroll 1
     for (int c0 = 0; c0 < live * kWidth; c0 += kAhead) {
       const T* p[kAhead];
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) p[n] = c0 + n < columns ? row(c0 + n) : nullptr;
-      uint4* to = pieces + c0 / kWidth * units * kUnitPieces;
+      const int block = c0 / kWidth, col0 = c0 % kWidth;
+      uint4* to = pieces + block * units * kUnitPieces;
 #pragma unroll 1
       for (int i = threadIdx.x * 8; i < padded; i += blockDim.x * 8) {
-        uint4 v[kAhead];
+        uint4 v[kAhead][kParts];
 #pragma unroll
         for (int n = 0; n < kAhead; ++n)
-          v[n] = p[n] != nullptr && i < k ? *reinterpret_cast<const uint4*>(p[n] + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part)
+            v[n][part] = p[n] != nullptr && i < k ? *reinterpret_cast<const uint4*>(p[n] + part * k + i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int n = 0; n < kAhead; ++n) {
           if constexpr (W::kIs4 && !kSumProducts) {
             // the group's threads are neighbours (padded is whole warps)
-            const float2 a = MmaType<T>::unpack(v[n].x), b = MmaType<T>::unpack(v[n].y), c = MmaType<T>::unpack(v[n].z),
-                         d = MmaType<T>::unpack(v[n].w);
-            float sum = ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
+            float sum = 0.0f;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              const uint4 w = v[n][part];
+              const float2 a = MmaType<T>::unpack(w.x), b = MmaType<T>::unpack(w.y), c = MmaType<T>::unpack(w.z),
+                           d = MmaType<T>::unpack(w.w);
+              sum += ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
+            }
 #pragma unroll
             for (int o = W::kGroupK / 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (i % W::kGroupK == 0) sums[(c0 / kWidth * units * W::kSub + i / W::kGroupK) * 8 + n] = sum * Scaling<F, T>::kSum;
+            if (i % W::kGroupK == 0) sums[(block * units * W::kSub + i / W::kGroupK) * 8 + col0 + n] = sum * Scaling<F, T>::kSum;
           }
-          to[piece_index<F, kWidth>(i, n)] = piece_order<F, T>(v[n]);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part)
+            to[piece_index<F, kWidth, kParts>(i, col0 + n, part)] = piece_order<F, T>(v[n][part]);
         }
       }
     }
@@ -360,9 +373,12 @@ struct XTile {
           float sum[4] = {};
 #pragma unroll
           for (int q = j * W::kPieces / W::kSub; q < (j + 1) * W::kPieces / W::kSub; ++q) {
-            const uint4 x = piece(pieces + i * kUnitPieces, i % units, q);
-            MmaType<T>::mma(sum, kOne, kOne, kOne, kOne, x.x, x.y);
-            MmaType<T>::mma(sum, kOneOdd, kOneOdd, kOneOdd, kOneOdd, x.z, x.w);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              const uint4 x = piece(pieces + i * kUnitPieces, i % units, q, part);
+              MmaType<T>::mma(sum, kOne, kOne, kOne, kOne, x.x, x.y);
+              MmaType<T>::mma(sum, kOneOdd, kOneOdd, kOneOdd, kOneOdd, x.z, x.w);
+            }
           }
           if (lane < 4) *reinterpret_cast<float2*>(sums + (i * W::kSub + j) * 8 + 2 * lane) = make_float2(sum[0], sum[1]);
         }
@@ -372,9 +388,9 @@ struct XTile {
   }
 
   // The lane's piece j of unit u, whose pieces start at `at`.
-  __device__ __forceinline__ uint4 piece(const uint4* at, int u, int j) const {
+  __device__ __forceinline__ uint4 piece(const uint4* at, int u, int j, int part) const {
     const int lane = threadIdx.x & 31;
-    const uint4* p = at + j * kWidth * 4 + (lane ^ piece_swap<F>(u, j));
+    const uint4* p = at + (j * kParts + part) * kWidth * 4 + (lane ^ piece_swap<F>(u, j));
     if (kWidth == 8) return *p;
     return lane < kWidth * 4 ? *p : make_uint4(0, 0, 0, 0);
   }
@@ -391,9 +407,12 @@ struct XTile {
     if constexpr (F == kWBf16) {
 #pragma unroll
       for (int b = 0; b < NBL; ++b) {
-        const uint4 x = piece(at + b * units * kUnitPieces, u, 0);
-        M::mma(acc[b], w[0][0], w[1][0], w[0][1], w[1][1], x.x, x.y);
-        M::mma(acc[b], w[0][2], w[1][2], w[0][3], w[1][3], x.z, x.w);
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+          const uint4 x = piece(at + b * units * kUnitPieces, u, 0, p);
+          M::mma(acc[b], w[0][0], w[1][0], w[0][1], w[1][1], x.x, x.y);
+          M::mma(acc[b], w[0][2], w[1][2], w[0][3], w[1][3], x.z, x.w);
+        }
       }
     } else {
       if constexpr (W::kIs4) {
@@ -426,9 +445,12 @@ struct XTile {
           }
 #pragma unroll
           for (int b = 0; b < NBL; ++b) {
-            const uint4 x = piece(at + b * units * kUnitPieces, u, j);
-            M::mma(part[b], a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
-            M::mma(kApart ? odd[b] : part[b], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+              const uint4 x = piece(at + b * units * kUnitPieces, u, j, p);
+              M::mma(part[b], a[0][0], a[1][0], a[0][1], a[1][1], x.x, x.y);
+              M::mma(kApart ? odd[b] : part[b], a[0][2], a[1][2], a[0][3], a[1][3], x.z, x.w);
+            }
           }
         }
         float s[2], z[2];
