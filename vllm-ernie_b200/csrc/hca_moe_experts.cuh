@@ -188,13 +188,23 @@ struct Shape {
   int room;                  // bytes for columns
 };
 
+// Columns of the products.  h comes in two parts: where a block has room for
+// them the second parts are columns of their own, kWidth after the first, and
+// cost no product; else each weight's fragment meets both.
+template <int F, int NB, int kWidth, int kParts, bool kUp>
+struct Columns {
+  static constexpr bool kBeside = !kUp && kParts == 2 && kWidth < 8;
+  using X = XTile<F, __nv_bfloat16, NB, kBeside ? 2 * kWidth : kWidth, kUp || kBeside ? 1 : kParts>;
+};
+
 // One of the products over this CTA's run of (entry, tile) items.  kUp: h from
 // x (fragment rows 0..7 of a tile are gate rows, 8..15 the up rows of the same
 // inner columns, so a lane holds both factors); else part from h.
 template <int F, int NB, int kWidth, int kParts, bool kUp>
 struct Product {
   using W = WTraits<F>;
-  using X = XTile<F, __nv_bfloat16, NB, kWidth, kUp ? 1 : kParts>;
+  static constexpr bool kBeside = Columns<F, NB, kWidth, kParts, kUp>::kBeside;
+  using X = typename Columns<F, NB, kWidth, kParts, kUp>::X;
   using P = Plan<NB * kWidth>;
   const MoePass& p;
   const MoeWeights& w;
@@ -361,11 +371,13 @@ struct Product {
     for (int entry = first_entry; entry <= end_at.entry; ++entry) {
       const int l0 = pl.start[entry];
       X xt(smem + (entry - first_entry) * tile_bytes, W::units(k));
-      xt.stage(k, dense ? p.tokens : pl.start[entry + 1] - l0, most, [&](int col) -> const __nv_bfloat16* {
+      const int n = dense ? p.tokens : pl.start[entry + 1] - l0;
+      xt.stage(k, kBeside ? kWidth + n : n, most, [&](int col) -> const __nv_bfloat16* {
         if (kUp && dense)
           return p.routing.mask == nullptr || p.routing.mask[col] ? p.x + col * p.x_stride : nullptr;
-        const int pair = pl.pair[l0 + col];
-        return kUp ? p.x + token(pair) * p.x_stride : h_row(pair);
+        if (kBeside && col % kWidth >= n) return nullptr;
+        const int pair = pl.pair[l0 + (kBeside ? col % kWidth : col)];
+        return kUp ? p.x + token(pair) * p.x_stride : h_row(pair) + (kBeside && col >= kWidth ? k : 0);
       });
     }
     X xt(smem, W::units(k));
@@ -381,7 +393,8 @@ struct Product {
       for (int i = g.thread(); i < n; i += g.threads()) {
         const int pair = pl.pair[s0 + i / kCols], c = i % kCols;
         const int col = dense ? token(pair) : i / kCols;
-        const float v = TileSums<NB>::sum(sums, g, c, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
+        float v = TileSums<NB>::sum(sums, g, c, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
+        if (kBeside) v += TileSums<NB>::sum(sums, g, c, 0, kWidth + col) * Scaling<F, __nv_bfloat16>::kOut;
         if (kUp) {
           const float up = TileSums<NB>::sum(sums, g, c + 8, col / kWidth, col % kWidth) * Scaling<F, __nv_bfloat16>::kOut;
           const float h = __fdividef(v, 1.0f + __expf(-v)) * up * pl.weight[pair];
@@ -469,8 +482,8 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
                                  static_cast<int64_t>(p.hidden / 16) * W::units(inner));
   if (units * p.tokens * (p.routing.top_k + 1) > UINT32_MAX) return false;
   Shape shape;
-  shape.room = static_cast<int>(std::max(XTile<F, __nv_bfloat16, NB, kWidth>::bytes(W::units(p.hidden)),
-                                         XTile<F, __nv_bfloat16, NB, kWidth, kParts>::bytes(W::units(inner))));
+  shape.room = static_cast<int>(std::max(Columns<F, NB, kWidth, kParts, true>::X::bytes(W::units(p.hidden)),
+                                         Columns<F, NB, kWidth, kParts, false>::X::bytes(W::units(inner))));
   const int64_t columns = shape.room + TileSums<NB>::bytes(kWarps);
   const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr;
   auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
