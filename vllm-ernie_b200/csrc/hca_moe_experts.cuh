@@ -484,6 +484,12 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   Shape shape;
   shape.room = static_cast<int>(std::max(Columns<F, NB, kWidth, kParts, true>::X::bytes(W::units(p.hidden)),
                                          Columns<F, NB, kWidth, kParts, false>::X::bytes(W::units(inner))));
+  // Columns of h of the experts that a CTA's run meets, as long as they are
+  // small: a second layout costs a small layer 3 us of 18, but loads on their
+  // way need what shared memory leaves of L1.
+  const int64_t meets = cdiv(std::min(p.routing.experts, p.tokens * p.routing.top_k), sms) + 1;
+  const int64_t met = meets * Columns<F, NB, kWidth, kParts, false>::X::bytes(W::units(p.inner));
+  shape.room = static_cast<int>(std::max<int64_t>(shape.room, std::min<int64_t>(met, 64 * 1024)));
   const int64_t columns = shape.room + TileSums<NB>::bytes(kWarps);
   const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr;
   auto scales = [&](int k, int warps) { return ScaleTile<F>::bytes(W::units(k), zeros, warps, kWarps); };
