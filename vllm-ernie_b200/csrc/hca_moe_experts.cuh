@@ -9,16 +9,19 @@
 // few experts and lays out their columns in shared memory once.  The second
 // product leaves each (token, slot) pair's share of y in 32 bits, and the last
 // step adds a token's shares in the order of its slots: no atomics, and a
-// token's result depends on how many others are in the batch, not on which.  h is rounded
-// to bf16 once, its weight included.
+// token's result depends on how many others are in the batch, not on which.  h,
+// its weight included, is kept as two bf16 numbers, rounded and rest: with one,
+// results were 1.4 to 1.6 times as far from the definition as with 32 bits
+// between the products (0.0024 for 0.0017, the rounding of the result itself),
+// for 5 to 7 % less time with more than four tokens and none with fewer.
 //
 // One launch with two grid barriers, since each of the steps is short at one
 // token: the weights of the second product start on their way before the
 // barrier that its activations wait for.
 //
 // Measured, router and all: e4m3, 8 tokens, 8 of 128 experts, 4096 x 1024 and a
-// shared one: 113 us, 5.9 TB/s; bf16, one token, 6 of 64: 37.4 us, 4.0 TB/s;
-// 4-bit, 64 tokens, 8 of 128: 187 us, 4.4 TB/s, bound by latency at 16 warps an
+// shared one: 118 us, 5.6 TB/s; bf16, one token, 6 of 64: 37.9 us, 4.0 TB/s;
+// 4-bit, 64 tokens, 8 of 128: 193 us, 4.2 TB/s, bound by latency at 16 warps an
 // SM (weights and the groups' barriers are two fifths of what warps wait for).
 // Of a small layer's 18 us (4-bit, 2 tokens, 4 of 32, 1024 x 512), 3 are the
 // router, 3 the plan, 3 1/2 the starts of the products, 6 the products and 2 1/2
@@ -542,8 +545,8 @@ int moe_experts_pass(const MoePass& p, const MoeWeights& w, cudaStream_t s) {
   // Columns of an entry, where shared memory holds them: two blocks of eight if
   // an expert gets more than eight tokens on average, or all tokens fit and it
   // gets more than two; else one, which an expert with more tokens passes
-  // several times (at 64 tokens, four an expert, 188 us for 226 with 4-bit
-  // weights, 96 for 106 with e4m3; at 12 tokens, three an expert, 40 for 34 and
+  // several times (with h in one part, at 64 tokens, four an expert, 188 us for 226
+  // with 4-bit weights, 96 for 106 with e4m3; at 12 tokens, three an expert, 40 for 34 and
   // 47 for 41).  bf16 weights, with nothing to unpack, gain from two blocks
   // whenever there are more than eight tokens (58 us for 47 at 12 tokens).
   int rc = HCA_OK;

@@ -12,7 +12,7 @@
 // 5.2 TB/s (a run of seconds meets the power limit: 61 us at 1.65 GHz; the loop
 // keeps the issue slots half and the shared-memory pipe two thirds busy).  Small
 // ones are bound by what comes before the first product, laying out x above all
-// (16 rows of 4096: 2.9 us of 10.6 for [8192, 4096]), and with groups of 32 by
+// (16 rows of 4096: about 2 us of 10.0 for [8192, 4096]), and with groups of 32 by
 // the unpacking (fp16, [4096, 8192], 3 rows: 10.1 us); [8192, 1024], one row:
 // 3.8 us.
 #include "hca_stream.cuh"

@@ -816,8 +816,8 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
     experts of another rank; an id may repeat), ``weights`` fp32 ``[T, top_k]``.
     Each chosen expert's weights are read once for all its tokens (of 64 at a
     time; again for each 16 tokens of one expert).  Rows that ``token_mask``
-    leaves out come out as 0 and choose nothing.  The gated product is rounded
-    to bf16 once, its weight included; sums are fp32."""
+    leaves out come out as 0 and choose nothing.  The gated product, its
+    weight included, is kept in two bf16 parts (16 bits); sums are fp32."""
     dev, t, hidden, stride, at = _moe_rows(x, token_mask, ids, weights)
     fmt, group, ptrs, num, inner, shared_inner = _moe_args(hidden, dev, experts, shared)
     if (ids.dtype is not _I32 or ids.dim() != 2 or ids.shape[0] != t or not ids.is_contiguous()
