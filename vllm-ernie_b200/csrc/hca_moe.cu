@@ -5,8 +5,8 @@
 //   weights[t, j] = p[t, ids[t, j]] (/ their sum) * scale
 //
 // The logits are latency-bound (experts * hidden weights, a few MB at most),
-// so they are spread over the whole GPU: a CTA computes two experts
-// for up to eight tokens, its warps splitting hidden.  Products and sums are
+// so they are spread over the whole GPU: a CTA computes two experts for up to
+// eight tokens, its warps splitting hidden.  Products and sums are
 // 32-bit multiply-adds: a bf16 tensor product would make near-ties of a 32-bit
 // router fall differently.  The choice itself is one warp's work a token, and up
 // to 16 tokens every CTA of the expert kernel makes it for itself.  About 3 us

@@ -1,7 +1,8 @@
 // Shared by the kernels of the few-token mixture-of-experts layer.
 //
-// A call is two launches.  The first computes the router's logits over the
-// whole GPU and clears the second's barrier; the second, one CTA an SM,
+// A call is two launches (above 16 tokens a third between them chooses the
+// experts).  The first computes the router's logits over the whole GPU and
+// clears the second's barrier; the second, one CTA an SM,
 // resident together, chooses the experts, runs both of their products and adds
 // up the result, with a grid barrier between the steps.
 #pragma once
