@@ -14,9 +14,10 @@
 // few hundred and its lanes share them out, so that their loads run together.
 //
 // Bound by scattered accesses of a sector for two or four bytes.  Measured: 192
-// rows of 151937 bf16 logits with histories up to 32768: 55 us (75 MB of sectors
-// each way; two fifths of a CTA's time go into clearing its tables and counting,
-// which nothing overlaps, one CTA filling an SM's shared memory); 64 rows of 129280 fp32 logits with masks: 15.5 us; one
+// rows of 151937 bf16 logits with histories up to 32768: 55 us (47 MB of sectors
+// read and written, 25 MB of histories; two fifths of a CTA's time go into
+// clearing its tables and counting, which nothing overlaps, one CTA filling an
+// SM's shared memory); 64 rows of 129280 fp32 logits with masks: 15.5 us; one
 // row with a short history: 3.5 us.
 #include <algorithm>
 

@@ -815,7 +815,7 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
     ``ids`` int32 ``[T, top_k]`` (ids outside ``[0, E)`` are skipped, as for the
     experts of another rank; an id may repeat), ``weights`` fp32 ``[T, top_k]``.
     Each chosen expert's weights are read once for all its tokens (of 64 at a
-    time; again for each 16 tokens of one expert).  Rows that ``token_mask``
+    time; again for each 8 or 16 tokens of one expert).  Rows that ``token_mask``
     leaves out come out as 0 and choose nothing.  The gated product, its
     weight included, is kept in two bf16 parts (16 bits); sums are fp32."""
     dev, t, hidden, stride, at = _moe_rows(x, token_mask, ids, weights)
