@@ -336,7 +336,8 @@ struct Product {
     first = {first_entry, tile};
     move(first, g.id);
     loading = fetching = now = first;
-    stream.start(k_of(first_entry), g, to - from > g.id ? (to - from - g.id + per_cta - 1) / per_cta : 0, scale_smem, *this);
+    const int k = k_of(first_entry);
+    stream.start(k, g, to - from > g.id ? (to - from - g.id + per_cta - 1) / per_cta : 0, scale_smem, *this, W::units(k));
     return true;
   }
 

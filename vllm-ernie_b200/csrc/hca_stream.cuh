@@ -574,9 +574,11 @@ struct TileStream {
     }
   }
   // Starts the loads of `count` tiles of rows of k, this warp's share of each;
-  // `smem` is for the scales, of ScaleTile::bytes(units, ...) at most.
+  // `smem` is for the scales, of ScaleTile::bytes(units, ...) at most.  Runs
+  // that no block barrier parts have to name the same `scale_units`, those of
+  // the longest: the warps' areas lie by it, and one warp may be a run ahead.
   template <typename Source>
-  __device__ __forceinline__ void start(int k_, const TileGroup& g, int count_, uint8_t* smem, Source& source) {
+  __device__ __forceinline__ void start(int k_, const TileGroup& g, int count_, uint8_t* smem, Source& source, int scale_units) {
     const int units = W::units(k_);
     k = k_, u0 = g.first_unit(units), u1 = g.end_unit(units), count = count_;
     if (count > 0) {
@@ -585,7 +587,7 @@ struct TileStream {
     }
     if constexpr (W::kIs4) {
       g0 = min(u0 * W::kSub, k / W::kGroupK), g1 = min(u1 * W::kSub, k / W::kGroupK);
-      sc.init(smem, units, source.zeros(), g.warps, source.rows_wide(), g0, g1);
+      sc.init(smem, scale_units, source.zeros(), g.warps, source.rows_wide(), g0, g1);
       __syncwarp();  // the last run's scales have been read
       fetch_scales(0, source);
       fetch_scales(1, source);

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_linear_kernel(W4Args a) {
   pdl_wait_and_release();
   TileStream<F, T, WTraits<F>::step(NB)> stream;
   stream.start(a.k, g, src.first < tiles ? (tiles - src.first + src.stride - 1) / src.stride : 0,
-             smem + X::bytes(units) + TileSums<NB>::bytes(kWarps), src);
+             smem + X::bytes(units) + TileSums<NB>::bytes(kWarps), src, units);
   const T* x = static_cast<const T*>(a.x) + t0 * a.x_stride;
   xt.stage(a.k, columns, live, [&](int col) { return x + col * a.x_stride; });
 
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) w4_long_kernel(W4Args a) {
     for (; src.k0 < a.k; src.k0 += kLongK) {
       const int k = min(kLongK, a.k - src.k0);
       TileStream<F, T, W::step(1)> stream;
-      stream.start(k, g, mine, scales, src);
+      stream.start(k, g, mine, scales, src, units);  // other groups may still read the last piece's scales
       __syncthreads();  // the last piece has been read
       X xt(smem, W::units(k));
       xt.stage(k, columns, 1, [&](int col) { return x + col * a.x_stride + src.k0; });
