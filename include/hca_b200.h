@@ -486,8 +486,7 @@ int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride,
  * aligned.  ids outside
  * [0, E) are skipped; an id that repeats in a row counts with its weights' sum.  A row whose token_mask byte is 0
  * takes no part and its out is 0.  I, Is and H multiples of 32 (and of the
- * group).  The gated product, with its weight in it, is kept in two bf16 parts
- * (in one where I or Is is too long for shared memory, above 16 thousand or so);
+ * group).  The gated product, with its weight in it, is kept in two bf16 parts;
  * everything else is summed in fp32.  Any T; passes of 64 tokens.
  * workspace: hca_moe_workspace_bytes(...) bytes, 16-byte aligned, not to be
  * shared by calls that are not ordered on one stream. */

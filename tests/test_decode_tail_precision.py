@@ -21,6 +21,7 @@ import torch
 
 gpu = pytest.mark.gpu
 
+FP8 = torch.float8_e4m3fn
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
@@ -95,6 +96,20 @@ def test_the_long_row_check_tells_mistakes_apart(group, k, dtype):
     assert not holds(part.to(dtype) + (ref - part).to(dtype))  # rounded between the pieces
 
 
+@pytest.mark.parametrize("inner", [128, 384, 16384])
+def test_the_rounding_check_tells_one_bf16_number_from_two(inner):
+    gen = torch.Generator().manual_seed(2)
+    h = torch.randn((3, inner), generator=gen).double()
+    w2 = torch.randn((1024, inner), generator=gen).double()
+    ref = h @ w2.T
+    first = h.bfloat16()
+    second = (h - first.double()).bfloat16()
+    assert _rounded_once(((first.double() + second.double()) @ w2.T).bfloat16(), ref, torch.bfloat16)
+    assert not _rounded_once((first.double() @ w2.T).bfloat16(), ref, torch.bfloat16)
+    swapped = first.double() + second.double().roll(1, 0)  # another token's second part
+    assert not _rounded_once((swapped @ w2.T).bfloat16(), ref, torch.bfloat16)
+
+
 # ---------------------------------------------------------------------------
 # 4-bit products of long rows
 # ---------------------------------------------------------------------------
@@ -121,3 +136,81 @@ def test_w4_linear_of_long_rows(tokens, n, k, group, zeros, dtype):
     assert _w4_holds(got[0], ref, size, dtype, k // group)
     for again in got[1:]:
         assert torch.equal(again, got[0])
+
+
+# ---------------------------------------------------------------------------
+# experts
+# ---------------------------------------------------------------------------
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _matrix(kind, shape, gen):
+    """(data, scales, zero points, 64-bit weights) of a weight format."""
+    *lead, n, k = shape
+    if kind.startswith("w4"):
+        group, zeros = int(kind.split("-")[1].rstrip("z")), kind.endswith("z")
+        q, s, z = _w4_weights(math.prod(lead) * n, k, group, zeros, torch.bfloat16, gen, "cuda")
+        w = _w4_rows(q, s, z, group).view(shape)
+        return q.view(*lead, n, -1), s.view(*lead, n, -1), None if z is None else z.view(*lead, n, -1), w
+    w = torch.randn(shape, generator=gen, device="cuda") / math.sqrt(k)
+    if kind == "bf16":
+        return w.bfloat16(), None, None, w.bfloat16().double()
+    s = torch.exp2(torch.randint(-3, 1, (*lead, -(-n // 128), -(-k // 128)), generator=gen, device="cuda").float()) / 37
+    d = (w * 37).to(FP8)
+    return d, s, None, d.double() * s.double().repeat_interleave(128, -2).repeat_interleave(128, -1)[..., :n, :k]
+
+
+def _stack(kind, lead, hidden, inner, gen):
+    d13, s13, z13, w13 = _matrix(kind, (*lead, 2 * inner, hidden), gen)
+    d2, s2, z2, w2 = _matrix(kind, (*lead, hidden, inner), gen)
+    return _ops().MoEWeights(d13, d2, s13, s2, z13, z2), w13, w2
+
+
+def _mlp(x, w13, w2):
+    gate, up = (x @ w13.transpose(-1, -2)).chunk(2, -1)
+    return (gate * torch.sigmoid(gate) * up) @ w2.transpose(-1, -2)
+
+
+def _experts_ref(x, ids, weights, w13, w2, shared=None):
+    x, weights = x.double(), weights.double()
+    y = torch.zeros_like(x) if shared is None else _mlp(x, *shared)
+    for e in range(w13.shape[0]):
+        t, j = torch.nonzero(ids == e, as_tuple=True)
+        y.index_add_(0, t, _mlp(x[t], w13[e], w2[e]) * weights[t, j].unsqueeze(1))
+    return y
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "w4-32", "w4-64z", "w4-128"])
+@pytest.mark.parametrize("tokens,experts,hidden,inner,shared", [
+    (1, 4, 1024, 256, 384), (2, 4, 1024, 384, 128), (3, 4, 1024, 256, 384), (4, 6, 1024, 384, 128), (5, 6, 1024, 256, 384),
+    (8, 6, 512, 384, 640), (9, 20, 512, 256, 384), (16, 3, 512, 384, 256), (40, 6, 512, 256, 384), (70, 12, 512, 128, 0)])
+def test_moe_experts_round_once(tokens, experts, hidden, inner, shared, kind):
+    """The gated product between the two products is not rounded to bf16: with it
+    in one number the error is that of two roundings.  All widths of columns, with
+    a shared expert of another length."""
+    gen = _gen(tokens + inner)
+    x = torch.randn((tokens, hidden), generator=gen, device="cuda").bfloat16()
+    stack, w13, w2 = _stack(kind, (experts,), hidden, inner, gen)
+    one, a, b = _stack(kind, (), hidden, shared, gen) if shared else (None, None, None)
+    ids = torch.rand((tokens, experts), generator=gen, device="cuda").argsort(1)[:, :3].int().contiguous()
+    weights = torch.rand((tokens, 3), generator=gen, device="cuda")
+    got = _ops().moe_experts(x, ids, weights, stack, shared=one)
+    assert _rounded_once(got, _experts_ref(x, ids, weights, w13, w2, (a, b) if shared else None), torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "w4-32", "w4-32z", "w4-64z", "w4-128z"])
+@pytest.mark.parametrize("tokens,inner,shared", [(1, 16384, 0), (5, 16384, 256), (3, 256, 16384), (9, 14336, 64 * 6)])
+def test_moe_experts_round_once_whatever_the_length(tokens, inner, shared, kind):
+    gen = _gen(tokens + inner)
+    x = torch.randn((tokens, 2048), generator=gen, device="cuda").bfloat16()
+    stack, w13, w2 = _stack(kind, (2,), 2048, inner, gen)
+    one, a, b = _stack(kind, (), 2048, shared, gen) if shared else (None, None, None)
+    ids = torch.randint(0, 2, (tokens, 1), generator=gen, device="cuda", dtype=torch.int32)
+    weights = torch.rand((tokens, 1), generator=gen, device="cuda") + 0.5
+    got = _ops().moe_experts(x, ids, weights, stack, shared=one)
+    assert _rounded_once(got, _experts_ref(x, ids, weights, w13, w2, (a, b) if shared else None), torch.bfloat16)

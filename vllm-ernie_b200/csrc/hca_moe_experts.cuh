@@ -40,6 +40,7 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 // shared memory of a CTA for columns and tile sums, beside the plan
 constexpr int64_t kSmem = 208 * 1024;
+constexpr int kParts = 2;  // bf16 numbers that an h is kept as
 constexpr int64_t kPrefetch = 256 * 1024;  // weights of a CTA on their way into L2 at the grid barrier
 static_assert(kWarps * 64 > kMoeExperts, "the plan's lanes hold two experts each");
 
@@ -51,7 +52,7 @@ static_assert(kWarps * 64 > kMoeExperts, "the plan's lanes hold two experts each
 // (number `experts`) last, and pairs in the tokens'.
 template <int kColumns>
 struct Plan {
-  static constexpr int kEntries = kMoeExperts + 1 + kMoePairs / kColumns;
+  static constexpr int kEntries = kColumns == 1 ? kMoePairs : kMoeExperts + 1 + kMoePairs / kColumns;
   int entries, routed;          // with and without the shared expert's
   int16_t expert[kEntries];     // entry -> expert
   int16_t start[kEntries + 1];  // entry -> first pair
@@ -194,20 +195,20 @@ struct Shape {
 // Columns of the products.  h comes in two parts: where a block has room for
 // them the second parts are columns of their own, kWidth after the first, and
 // cost no product; else each weight's fragment meets both.
-template <int F, int NB, int kWidth, int kParts, bool kUp>
+template <int F, int NB, int kWidth, bool kUp>
 struct Columns {
-  static constexpr bool kBeside = !kUp && kParts == 2 && kWidth < 8;
+  static constexpr bool kBeside = !kUp && kWidth < 8;
   using X = XTile<F, __nv_bfloat16, NB, kBeside ? 2 * kWidth : kWidth, kUp || kBeside ? 1 : kParts>;
 };
 
 // One of the products over this CTA's run of (entry, tile) items.  kUp: h from
 // x (fragment rows 0..7 of a tile are gate rows, 8..15 the up rows of the same
 // inner columns, so a lane holds both factors); else part from h.
-template <int F, int NB, int kWidth, int kParts, bool kUp>
+template <int F, int NB, int kWidth, bool kUp>
 struct Product {
   using W = WTraits<F>;
-  static constexpr bool kBeside = Columns<F, NB, kWidth, kParts, kUp>::kBeside;
-  using X = typename Columns<F, NB, kWidth, kParts, kUp>::X;
+  static constexpr bool kBeside = Columns<F, NB, kWidth, kUp>::kBeside;
+  using X = typename Columns<F, NB, kWidth, kUp>::X;
   using P = Plan<NB * kWidth>;
   const MoePass& p;
   const MoeWeights& w;
@@ -405,10 +406,8 @@ struct Product {
           __nv_bfloat16* to = h_row(pair) + now.tile * 8 + c;
           const __nv_bfloat16 first = __float2bfloat16_rn(h);
           *to = first;
-          if (kParts == 2) {
-            const float rest = h - __bfloat162float(first);
-            to[now.entry >= pl.routed ? p.shared_inner : p.inner] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
-          }
+          const float rest = h - __bfloat162float(first);
+          to[now.entry >= pl.routed ? p.shared_inner : p.inner] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
         } else {
           p.part[static_cast<int64_t>(pair) * p.hidden + now.tile * 16 + c] = v;
         }
@@ -422,10 +421,11 @@ struct Product {
   }
 };
 
-template <int F, int NB, int kWidth, int kParts>
+template <int F, int NB, int kWidth>
 __global__ void __launch_bounds__(kThreads, 1)
     moe_layer_kernel(MoePass p, MoeWeights w, Shape shape) {
   __shared__ Plan<NB * kWidth> pl;
+  static_assert(sizeof(pl) + kSmem <= 227 * 1024, "shared memory of a block");
   extern __shared__ __align__(16) uint8_t smem[];
   build_plan(pl, p);
   TileStream<F, __nv_bfloat16, WTraits<F>::step(NB)> stream;
@@ -434,12 +434,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   TileSums<NB> ts(sums);
   uint8_t* scales = sums + TileSums<NB>::bytes(kWarps);
   {
-    Product<F, NB, kWidth, kParts, true> up(p, w, pl, smem, room, scales, shape.up_warps, shape.dense);
+    Product<F, NB, kWidth, true> up(p, w, pl, smem, room, scales, shape.up_warps, shape.dense);
     while (up.start(stream)) up.run(stream, ts);
   }
   grid_arrive(p.barrier);
   {
-    Product<F, NB, kWidth, kParts, false> down(p, w, pl, smem, room, scales, shape.down_warps, false);
+    Product<F, NB, kWidth, false> down(p, w, pl, smem, room, scales, shape.down_warps, false);
     bool more = down.start(stream);
     // bf16 weights come slower than they are used, so they go on coming while
     // the CTAs meet (38.8 -> 37.9 us at one token; 4-bit and e4m3 lost 0.5 %)
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Launches with entries of NB blocks of kWidth columns if shared memory holds them.
-template <int F, int NB, int kWidth, int kParts = 2>
+template <int F, int NB, int kWidth>
 bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   using W = WTraits<F>;
   const int sms = device_sm_count();
@@ -486,13 +486,13 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
                                  static_cast<int64_t>(p.hidden / 16) * W::units(inner));
   if (units * p.tokens * (p.routing.top_k + 1) > UINT32_MAX) return false;
   Shape shape;
-  shape.room = static_cast<int>(std::max(Columns<F, NB, kWidth, kParts, true>::X::bytes(W::units(p.hidden)),
-                                         Columns<F, NB, kWidth, kParts, false>::X::bytes(W::units(inner))));
+  shape.room = static_cast<int>(std::max(Columns<F, NB, kWidth, true>::X::bytes(W::units(p.hidden)),
+                                         Columns<F, NB, kWidth, false>::X::bytes(W::units(inner))));
   // Columns of h of the experts that a CTA's run meets, as long as they are
   // small: a second layout costs a small layer 3 us of 18, but loads on their
   // way need what shared memory leaves of L1.
   const int64_t meets = cdiv(std::min(p.routing.experts, p.tokens * p.routing.top_k), sms) + 1;
-  const int64_t met = meets * Columns<F, NB, kWidth, kParts, false>::X::bytes(W::units(p.inner));
+  const int64_t met = meets * Columns<F, NB, kWidth, false>::X::bytes(W::units(p.inner));
   shape.room = static_cast<int>(std::max<int64_t>(shape.room, std::min<int64_t>(met, 64 * 1024)));
   const int64_t columns = shape.room + TileSums<NB>::bytes(kWarps);
   const bool zeros = w.w13.zero != nullptr || w.w2.zero != nullptr;
@@ -523,7 +523,7 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   if (shape.up_warps == 0 || shape.down_warps == 0) return false;
   const int64_t smem = columns + std::max(scales(p.hidden, shape.up_warps), scales(inner, shape.down_warps));
   static bool done[kMaxDevices] = {};
-  rc = set_func_attr_once(moe_layer_kernel<F, NB, kWidth, kParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
+  rc = set_func_attr_once(moe_layer_kernel<F, NB, kWidth>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem, done);
   if (rc != HCA_OK) return true;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeCooperative;
@@ -535,7 +535,7 @@ bool launch(const MoePass& p, const MoeWeights& w, cudaStream_t s, int& rc) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  rc = cuda_status(cudaLaunchKernelEx(&cfg, moe_layer_kernel<F, NB, kWidth, kParts>, p, w, shape));
+  rc = cuda_status(cudaLaunchKernelEx(&cfg, moe_layer_kernel<F, NB, kWidth>, p, w, shape));
   return true;
 }
 
@@ -557,8 +557,9 @@ int moe_experts_pass(const MoePass& p, const MoeWeights& w, cudaStream_t s) {
   if (p.tokens > 4 && moe::launch<F, 1, 8>(p, w, s, rc)) return rc;
   if (p.tokens > 2 && moe::launch<F, 1, 4>(p, w, s, rc)) return rc;
   if (moe::launch<F, 1, 2>(p, w, s, rc)) return rc;
-  // rows of h too long for two parts: rounded to bf16 once
-  if (moe::launch<F, 1, 2, 1>(p, w, s, rc)) return rc;
+  // rows so long that shared memory has no room for the parts of two: a pass
+  // over an expert's weights for each of its tokens
+  if (moe::launch<F, 1, 1>(p, w, s, rc)) return rc;
   return HCA_E_UNSUPPORTED;
 }
 

@@ -165,9 +165,10 @@ __device__ __forceinline__ void by_group(uint32_t (&w)[4]) {
 // unit follow each other, each 4 kWidth lanes wide.  The lanes of a piece are
 // swapped around by `piece_swap`, so that eight threads that lay out
 // consecutive activations write to eight different bank groups.
-template <int F>
+// (A single column has no lanes to swap.)
+template <int F, int kWidth>
 __device__ __forceinline__ int piece_swap(int u, int j) {
-  return F == kWBf16 ? 4 * (u & 1) : F == kW4G128 ? 2 * j : 4 * (j & 1);
+  return kWidth == 1 ? 0 : F == kWBf16 ? 4 * (u & 1) : F == kW4G128 ? 2 * j : 4 * (j & 1);
 }
 template <int F, int kWidth, int kParts>
 __device__ __forceinline__ int piece_index(int k, int col, int part) {
@@ -179,7 +180,7 @@ __device__ __forceinline__ int piece_index(int k, int col, int part) {
   else if constexpr (F == kW4G128) c = r / 32, j = r / 8 % 4;
   else if constexpr (F == kW4G64) c = r / 32 % 2 + r / 16 % 2 * 2, j = r / 64 * 2 + r / 8 % 2;
   else c = r / 8 % 4, j = r / 32;
-  return ((u * W::kPieces + j) * kParts + part) * kWidth * 4 + ((col * 4 + c) ^ piece_swap<F>(u, j));
+  return ((u * W::kPieces + j) * kParts + part) * kWidth * 4 + ((col * 4 + c) ^ piece_swap<F, kWidth>(u, j));
 }
 
 // Eight consecutive activations in a piece's order, that in which weights come
@@ -390,7 +391,7 @@ struct XTile {
   // The lane's piece j of unit u, whose pieces start at `at`.
   __device__ __forceinline__ uint4 piece(const uint4* at, int u, int j, int part) const {
     const int lane = threadIdx.x & 31;
-    const uint4* p = at + (j * kParts + part) * kWidth * 4 + (lane ^ piece_swap<F>(u, j));
+    const uint4* p = at + (j * kParts + part) * kWidth * 4 + (lane ^ piece_swap<F, kWidth>(u, j));
     if (kWidth == 8) return *p;
     return lane < kWidth * 4 ? *p : make_uint4(0, 0, 0, 0);
   }
