@@ -474,7 +474,7 @@ int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride,
 
 /* Weight formats of the expert matrices. */
 #define HCA_WEIGHT_BF16 0 /* [E, N, K] bf16 */
-#define HCA_WEIGHT_FP8 1  /* e4m3 with fp32 scales [E, ceil(N / 128), ceil(K / 128)] of 128 x 128 blocks */
+#define HCA_WEIGHT_FP8 1  /* e4m3 with fp32 scales [E, ceil(N / 128), ceil(K / 128)] of 128 x 128 blocks; a NaN makes what its row gives NaN */
 #define HCA_WEIGHT_W4 2   /* 4-bit codes [E, N, K / 2], bf16 scales [E, N, K / g], zeros or NULL, as hca_w4_linear */
 
 /* Experts of a mixture-of-experts layer for a few tokens:

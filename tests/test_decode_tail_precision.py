@@ -214,3 +214,33 @@ def test_moe_experts_round_once_whatever_the_length(tokens, inner, shared, kind)
     weights = torch.rand((tokens, 1), generator=gen, device="cuda") + 0.5
     got = _ops().moe_experts(x, ids, weights, stack, shared=one)
     assert _rounded_once(got, _experts_ref(x, ids, weights, w13, w2, (a, b) if shared else None), torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("value", [0x7F, 0xFF])
+@pytest.mark.parametrize("tokens,hidden,inner", [(2, 256, 128), (5, 2080, 736), (12, 512, 256)])
+def test_an_e4m3_nan_is_a_nan(tokens, hidden, inner, value):
+    """In an expert's first product it makes the expert's tokens NaN, in the second
+    its row of the result; others keep their bits."""
+    gen = _gen(tokens)
+    x = torch.randn((tokens, hidden), generator=gen, device="cuda").bfloat16()
+    stack, _, _ = _stack("fp8", (4,), hidden, inner, gen)
+    ids = torch.randint(0, 4, (tokens, 1), generator=gen, device="cuda", dtype=torch.int32)
+    ids[0] = 2
+    ids[1] = 1
+    weights = torch.rand((tokens, 1), generator=gen, device="cuda")
+    clean = _ops().moe_experts(x, ids, weights, stack)
+    has = ids[:, 0] == 2
+    for k in (0, 77, hidden - 1):
+        for row in (0, inner - 1, 2 * inner - 3):
+            bad = stack.w13.clone()
+            bad.view(torch.uint8)[2, row, k] = value
+            got = _ops().moe_experts(x, ids, weights, stack._replace(w13=bad))
+            assert torch.isnan(got[has]).all() and torch.equal(got[~has], clean[~has])
+    for k in (0, inner - 1):
+        bad = stack.w2.clone()
+        bad.view(torch.uint8)[2, hidden - 9, k] = value
+        got = _ops().moe_experts(x, ids, weights, stack._replace(w2=bad))
+        want = clean.clone()
+        want[has, hidden - 9] = math.nan
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(0), want.nan_to_num(0))

@@ -62,6 +62,7 @@ struct Plan {
   uint64_t who[kMoeExperts + 1];  // expert -> its tokens
   int16_t list[kMoeExperts + 1];  // expert -> first pair
   int sums[kWarps];               // of 64 experts: pairs, and entries from bit 16 on
+  int nan;                        // e4m3: a tile of the segment has one
 };
 
 template <int kColumns>
@@ -95,6 +96,7 @@ __device__ __forceinline__ void build_plan(Plan<kColumns>& pl, const MoePass& p)
       pl.weight[i] = weight;
     }
   }
+  if (threadIdx.x == 0) pl.nan = 0;
   if (threadIdx.x < kMoeTokens) {
     const int t = threadIdx.x;
     const bool in = t < p.tokens && p.shared_inner > 0 && (mask == nullptr || mask[t]);
@@ -212,7 +214,7 @@ struct Product {
   using P = Plan<NB * kWidth>;
   const MoePass& p;
   const MoeWeights& w;
-  const P& pl;
+  P& pl;
   uint8_t *smem, *scale_smem;
   int room;  // bytes for columns
   TileGroup g;
@@ -225,7 +227,7 @@ struct Product {
     int entry, tile;
   } first, loading, fetching, now;
 
-  __device__ __forceinline__ Product(const MoePass& p_, const MoeWeights& w_, const P& pl_, uint8_t* smem_, int room_,
+  __device__ __forceinline__ Product(const MoePass& p_, const MoeWeights& w_, P& pl_, uint8_t* smem_, int room_,
                                      uint8_t* scale_smem_, int warps, bool dense_)
       : p(p_), w(w_), pl(pl_), smem(smem_), scale_smem(scale_smem_), room(room_), g(warps), dense(dense_) {
     per_cta = kWarps / g.warps;
@@ -306,6 +308,7 @@ struct Product {
     return scales_of(fetching, r);
   }
   __device__ __forceinline__ WScales here(int, int r) const { return scales_of(now, r); }
+  __device__ __forceinline__ void met_nan() { pl.nan = 1; }
 
   __device__ __forceinline__ __nv_bfloat16* h_row(int pair) const {
     return p.h + kParts * (pair < pairs ? static_cast<int64_t>(pair) * p.inner
@@ -417,6 +420,39 @@ struct Product {
     };
     if (NB > 1 && most == 1) stream.template run<1>(xt, g, ts, acc, *this, finish);
     else stream.template run<NB>(xt, g, ts, acc, *this, finish);
+    __syncthreads();
+    if (F == kWFp8 && pl.nan) spread_nans(stream.count);
+  }
+
+  // Looks for the NaN among the segment's e4m3 weights, a warp to a row, and
+  // makes what came of their rows NaN.  Ends with a block barrier.
+  __device__ __forceinline__ void spread_nans(int count) {
+    const int lane = threadIdx.x & 31, k = k_of(first_entry);
+    Place at = first;
+#pragma unroll 1
+    for (int i = 0; i < count; ++i, move(at, per_cta)) {
+      int64_t e;
+      const MoeMatrix& m = matrix(at, e);
+#pragma unroll 1
+      for (int r = g.index; r < 16; r += g.warps) {
+        const uint8_t* from = m.data + (e * rows_of(at.entry) + row(at, r)) * k;
+        uint32_t nans = 0;
+#pragma unroll 1
+        for (int b = lane * 4; b < k; b += 128) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(from + b);
+          nans |= (v ^ (v + 0x01010101u)) & 0x80808080u;
+        }
+        if (!__any_sync(0xffffffffu, nans)) continue;
+#pragma unroll 1
+        for (int j = pl.start[at.entry] + lane; j < pl.start[at.entry + 1]; j += 32) {
+          const int pair = pl.pair[j];
+          if (kUp) h_row(pair)[at.tile * 8 + r % 8] = __float2bfloat16_rn(NAN);
+          else p.part[static_cast<int64_t>(pair) * p.hidden + at.tile * 16 + r] = NAN;
+        }
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) pl.nan = 0;
     __syncthreads();
   }
 };
