@@ -450,6 +450,9 @@ int hca_fp8_grouped_gemm(void* out, int64_t out_stride_tok, int64_t out_stride_g
  * g = group_size 32, 64 or 128, dividing K.  Products and sums in fp32, one
  * rounding.  Any T is right; the weights are read again for every 16 rows
  * (fewer, where shared memory does not hold 16 rows of x).
+ * bf16 x are scaled by 2^80 on the way: |x| below 2^48, larger ones count as
+ * infinite; below 2^-73 a term may be off by 2^-96 of a scale.  An infinite or NaN x
+ * makes its row of out infinite or NaN and touches no other.
  * q starts on 16 bytes, scales and zeros on 4; out must not overlap x. */
 int hca_w4_linear(void* out, int64_t out_stride, const void* x, int64_t x_stride, const uint8_t* q,
                   const void* scales, const uint8_t* zeros, int32_t num_tokens, int32_t n, int32_t k,
@@ -487,7 +490,9 @@ int hca_moe_route(int32_t* ids, float* weights, const void* x, int64_t x_stride,
  * [0, E) are skipped; an id that repeats in a row counts with its weights' sum.  A row whose token_mask byte is 0
  * takes no part and its out is 0.  I, Is and H multiples of 32 (and of the
  * group).  The gated product, with its weight in it, is kept in two bf16 parts;
- * everything else is summed in fp32.  Any T; passes of 64 tokens.
+ * everything else is summed in fp32.  Any T; passes of 64 tokens.  With e4m3
+ * and 4-bit weights x and the gated product have the range of hca_w4_linear's
+ * bf16 x: from 2^48 on they count as infinite, and the token's out is infinite or NaN.
  * workspace: hca_moe_workspace_bytes(...) bytes, 16-byte aligned, not to be
  * shared by calls that are not ordered on one stream. */
 int64_t hca_moe_workspace_bytes(int32_t num_tokens, int32_t num_experts, int32_t top_k, int32_t hidden,

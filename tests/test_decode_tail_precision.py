@@ -244,3 +244,55 @@ def test_an_e4m3_nan_is_a_nan(tokens, hidden, inner, value):
         want = clean.clone()
         want[has, hidden - 9] = math.nan
         assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+
+
+# ---------------------------------------------------------------------------
+# the range of bf16 activations
+# ---------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("tokens,k", [(1, 640), (4, 1152), (8, 640), (11, 4096), (9, 29952)])
+def test_w4_linear_over_the_range_of_activations(tokens, k, group, zeros):
+    """Rows of sizes from 2^-40 to just below 2^48 are all as exact as any; from
+    2^48 on a value makes its own row infinite or NaN, never a wrong number."""
+    gen = _gen(tokens + k)
+    size = torch.tensor([45, 0, 47, 20, -40], device="cuda").repeat(3)[:tokens].float()
+    x = (torch.randn((tokens, k), generator=gen, device="cuda").clamp(-1.9, 1.9) * torch.exp2(size).unsqueeze(1)).bfloat16()
+    q, s, z = _w4_weights(2000, k, group, zeros, torch.bfloat16, gen, "cuda")
+    got = _ops().w4_linear(x, q, s, z)
+    ref, _ = _w4_ref(x, q, s, z, group)
+    for t in range(tokens):
+        assert _rounded_once(got[t], ref[t], torch.bfloat16)
+    for value in (2.0 ** 52, -2.0 ** 100, math.inf, -math.inf, math.nan):
+        bad = x.clone()
+        bad[tokens // 2, k // 3] = value
+        out = _ops().w4_linear(bad, q, s, z)
+        assert not torch.isfinite(out[tokens // 2]).any()
+        keep = [t for t in range(tokens) if t != tokens // 2]
+        assert torch.equal(out[keep], got[keep])
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "w4-32", "w4-64z", "w4-128"])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 6, 12, 30])
+def test_moe_experts_over_the_range_of_activations(tokens, kind):
+    gen = _gen(tokens)
+    size = torch.tensor([22, 0, -20, 10], device="cuda").repeat(8)[:tokens].float()  # products of two below 2^48
+    x = (torch.randn((tokens, 640), generator=gen, device="cuda").clamp(-3, 3) * torch.exp2(size).unsqueeze(1)).bfloat16()
+    stack, w13, w2 = _stack(kind, (5,), 640, 384, gen)
+    one, a, b = _stack(kind, (), 640, 256, gen)
+    ids = torch.rand((tokens, 5), generator=gen, device="cuda").argsort(1)[:, :3].int().contiguous()
+    weights = torch.rand((tokens, 3), generator=gen, device="cuda")
+    got = _ops().moe_experts(x, ids, weights, stack, shared=one)
+    ref = _experts_ref(x, ids, weights, w13, w2, (a, b))
+    for t in range(tokens):
+        assert _rounded_once(got[t], ref[t], torch.bfloat16), t
+    for value in (2.0 ** 52, math.inf, math.nan):
+        bad = x.clone()
+        bad[tokens // 2, 333] = value
+        out = _ops().moe_experts(bad, ids, weights, stack, shared=one)
+        assert not torch.isfinite(out[tokens // 2]).any()
+        keep = [t for t in range(tokens) if t != tokens // 2]
+        assert torch.equal(out[keep], got[keep])

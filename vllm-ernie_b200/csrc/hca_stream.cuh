@@ -41,9 +41,11 @@
 // moved into the low exponent and high mantissa bits of a bf16 is its value
 // times 2^-120, the subnormals with it.  bf16 activations are scaled by 2^80
 // when they are laid out, so that the products keep clear of both ends of the
-// 32-bit range for |x| from 2^-73 to 2^47, and the powers of two leave with the
-// finished sum.  An e4m3 NaN comes out as 480 that way, so the stream tells its
-// source of tiles that have one; an infinite x makes its row NaN.
+// 32-bit range, and the powers of two leave with the finished sum.  From 2^48 on
+// an activation becomes infinite that way, and so does, or NaN, what its row
+// gives; below 2^-73 terms lose bits.  (Columns laid out again without the
+// scaling where it overflows were right, but cost ordinary ones 3 to 6 %.)  An
+// e4m3 NaN comes out as 480, so the stream tells its source of tiles that have one.
 //
 // Zero points come off the group's sum: s (sum q x - z sum x), with sum x
 // known once per column and group, where taking z from every code costs half

@@ -612,7 +612,9 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
     ``x`` ``[T, K]`` bf16 or fp16; ``qweight`` uint8 ``[N, K / 2]`` (low nibble
     = even k); ``scales`` ``[N, K / g]`` of x's type, g = 32, 64 or 128;
     ``zeros`` uint8 ``[N, K / g]`` (None: 8).  ``w = (q - zero) * scale``, sums
-    in fp32, one rounding to x's type.  ``out`` must not overlap ``x``.  Right
+    in fp32, one rounding to x's type.  A bf16 ``|x|`` of 2^48 and more counts as
+    infinite, below 2^-73 terms lose bits; an infinite or NaN ``x`` makes its own
+    row infinite or NaN.  ``out`` must not overlap ``x``.  Right
     for any T, made for up to 16 rows (each 16 more read the weights again; a
     prompt's thousands belong on a dense product)."""
     # in line, as the shortest of these calls take the GPU 4 us
@@ -683,7 +685,10 @@ class MoEWeights(NamedTuple):
     * e4m3 with fp32 scales of 128 x 128 blocks, ``s13 [E, ceil(2 I / 128),
       ceil(H / 128)]``, ``s2 [E, ceil(H / 128), ceil(I / 128)]``;
     * uint8 4-bit codes ``[E, 2 I, H / 2]``, ``[E, H, I / 2]`` with bf16 group
-      scales and optional zero points, as ``w4_linear``."""
+      scales and optional zero points, as ``w4_linear``.
+
+    With e4m3 and 4-bit weights the layer's input and its gated product have the
+    range of ``w4_linear``'s bf16 ``x``: below 2^48."""
 
     w13: torch.Tensor
     w2: torch.Tensor
