@@ -296,3 +296,27 @@ def test_moe_experts_over_the_range_of_activations(tokens, kind):
         assert not torch.isfinite(out[tokens // 2]).any()
         keep = [t for t in range(tokens) if t != tokens // 2]
         assert torch.equal(out[keep], got[keep])
+
+
+# ---------------------------------------------------------------------------
+# router
+# ---------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts", [16, 60, 300])
+def test_route_weights_are_those_of_32_bit_functions(score, experts):
+    """One activation of 1 a token and logits of 11 bits, so that they and their
+    differences are exact.  What rounds, in units of 2^-24: the exponential (2), a
+    sum of up to 300 of them (2 of the terms, 10 additions of a lane and 5 of the
+    tree), the division (1): 20 units, and in the subnormals one of their steps for
+    the exponential and one for the division."""
+    gen = _gen(4)
+    wr = torch.randint(-60 * 16, 60 * 16, (experts, 32), generator=gen, device="cuda") / 16.0
+    x = torch.eye(32, device="cuda").bfloat16()
+    ids, w = _ops().moe_route(x, wr, 16, score=score, renormalize=False)
+    l = wr.T.double()
+    p = torch.softmax(l, 1) if score == "softmax" else torch.sigmoid(l)
+    want = torch.gather(p, 1, ids.long())
+    assert ((w.double() - want).abs() <= 20 * 2.0 ** -24 * want + 2 * 2.0 ** -149).all()
