@@ -320,3 +320,22 @@ def test_route_weights_are_those_of_32_bit_functions(score, experts):
     p = torch.softmax(l, 1) if score == "softmax" else torch.sigmoid(l)
     want = torch.gather(p, 1, ids.long())
     assert ((w.double() - want).abs() <= 20 * 2.0 ** -24 * want + 2 * 2.0 ** -149).all()
+
+
+# ---------------------------------------------------------------------------
+# logits
+# ---------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("value", [1.1, 0.7, 3.0, 2.0 ** -130])
+def test_the_repetition_penalty_divides(value):
+    """fp32 logits have the bits of the division and the product of the definition
+    (the reciprocal of a penalty below 2^-128 is infinite, quotients are not)."""
+    x = torch.randn((4, 5000), generator=_gen(3), device="cuda") * (2.0 ** -20 if value < 1e-30 else 5.0)
+    ids = torch.arange(5000, device="cuda", dtype=torch.int32).repeat(4, 1)
+    lens = torch.full((4,), 5000, device="cuda", dtype=torch.int32)
+    r = torch.full((4,), value, device="cuda")
+    want = torch.where(x > 0, x / r[:, None], x * r[:, None])
+    assert torch.isfinite(want).all()
+    assert torch.equal(_ops().apply_logit_penalties(x, ids, lens, lens, repetition=r), want)

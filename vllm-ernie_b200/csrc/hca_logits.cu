@@ -144,10 +144,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logit_penalty_kerne
   }
   __syncthreads();
 
-  const float inverse = 1.0f / rep;
   const int32_t* allowed = a.allowed == nullptr ? nullptr : a.allowed + row * a.allowed_stride;
   auto penalise = [&](float x, uint32_t n, bool seen) {
-    if (seen) x = x * (x > 0.0f ? inverse : rep);
+    if (seen) x = x > 0.0f ? x / rep : x * rep;
     if (n != 0) x = x - freq * static_cast<float>(n) - pres;
     return x;
   };
