@@ -339,3 +339,26 @@ def test_the_repetition_penalty_divides(value):
     want = torch.where(x > 0, x / r[:, None], x * r[:, None])
     assert torch.isfinite(want).all()
     assert torch.equal(_ops().apply_logit_penalties(x, ids, lens, lens, repetition=r), want)
+
+
+# ---------------------------------------------------------------------------
+# more rows than a grid has columns
+# ---------------------------------------------------------------------------
+
+
+@gpu
+def test_w4_linear_of_very_many_rows():
+    gen = _gen(1)
+    x = torch.randn((65536 + 70, 32), generator=gen, device="cuda").bfloat16()
+    q, s, z = _w4_weights(16, 32, 32, True, torch.bfloat16, gen, "cuda")
+    got = _ops().w4_linear(x, q, s, z)
+    assert torch.equal(got[65530:], _ops().w4_linear(x[65530:], q, s, z)) and torch.equal(got[:9], _ops().w4_linear(x[:9], q, s, z))
+
+
+@gpu
+def test_moe_route_of_very_many_rows():
+    x = torch.randn((65536 * 8 + 20, 32), generator=_gen(1), device="cuda").bfloat16()
+    wr = torch.randn((3, 32), generator=_gen(2), device="cuda")
+    ids, w = _ops().moe_route(x, wr, 2)
+    last, lw = _ops().moe_route(x[-40:], wr, 2)
+    assert torch.equal(ids[-40:], last) and torch.equal(w[-40:], lw)

@@ -146,7 +146,6 @@ bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) %
 int check_sizes(int tokens, int experts, int hidden, int top_k) {
   HCA_CHECK_ARG(tokens >= 0 && experts > 0 && hidden > 0 && top_k > 0 && top_k <= experts);
   if (experts > kMoeExperts || top_k > kMoeTopK || hidden % 32 != 0) return HCA_E_UNSUPPORTED;
-  HCA_CHECK_ARG(cdiv(tokens, 8) <= 65535);
   return HCA_OK;
 }
 
@@ -157,11 +156,18 @@ int check_rows(const void* x, int64_t x_stride) {
 
 int compute_logits(float* logits, const void* x, int64_t x_stride, const void* router, int router_fp32, int tokens,
                    int experts, int hidden, uint32_t* barriers, int num_barriers, cudaStream_t s) {
-  return router_fp32
-             ? logits_by_tokens<float>(tokens, logits, x, x_stride, router, tokens, experts, hidden, barriers,
-                                       num_barriers, s)
-             : logits_by_tokens<__nv_bfloat16>(tokens, logits, x, x_stride, router, tokens, experts, hidden, barriers,
-                                               num_barriers, s);
+  // a launch for each 524280 tokens, a grid's 65535 eights; the first clears the barriers
+  constexpr int kTokens = 8 * 65535;
+  for (int t = 0; t < tokens; t += std::min(kTokens, tokens - t)) {
+    const int n = std::min(kTokens, tokens - t), clear = t == 0 ? num_barriers : 0;
+    float* to = logits + static_cast<int64_t>(t) * experts;
+    const void* from = static_cast<const uint16_t*>(x) + t * x_stride;
+    const int rc = router_fp32
+                       ? logits_by_tokens<float>(n, to, from, x_stride, router, n, experts, hidden, barriers, clear, s)
+                       : logits_by_tokens<__nv_bfloat16>(n, to, from, x_stride, router, n, experts, hidden, barriers, clear, s);
+    if (rc != HCA_OK) return rc;
+  }
+  return HCA_OK;
 }
 
 int64_t align_up(int64_t v) { return (v + 255) / 256 * 256; }

@@ -232,8 +232,15 @@ extern "C" int hca_w4_linear(void* out, int64_t out_stride, const void* x, int64
   HCA_CHECK_ARG(x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0);
   HCA_CHECK_ARG(reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0 &&
                 reinterpret_cast<uintptr_t>(zeros) % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 2 == 0);
-  HCA_CHECK_ARG(num_tokens <= 65535 && n <= INT32_MAX - 16);  // grid columns hold at least one row of x
-  W4Args a{out, out_stride, x, x_stride, q, scales, zeros, num_tokens, n, k, 1, 0};
+  HCA_CHECK_ARG(n <= INT32_MAX - 16);
   cudaStream_t s = as_stream(stream);
-  return is_fp16 ? by_group<__half>(group_size, a, s) : by_group<__nv_bfloat16>(group_size, a, s);
+  // a launch for each 65520 rows (whole blocks of columns): a grid has 65535 at most
+  constexpr int kRows = 65520;
+  for (int t = 0; t < num_tokens; t += std::min(kRows, num_tokens - t)) {
+    const W4Args a{static_cast<uint16_t*>(out) + t * out_stride, out_stride, static_cast<const uint16_t*>(x) + t * x_stride,
+                   x_stride, q, scales, zeros, std::min(kRows, num_tokens - t), n, k, 1, 0};
+    const int rc = is_fp16 ? by_group<__half>(group_size, a, s) : by_group<__nv_bfloat16>(group_size, a, s);
+    if (rc != HCA_OK) return rc;
+  }
+  return HCA_OK;
 }
