@@ -84,9 +84,11 @@ class DecodeTail:
                                          bias_ids=self.bias_ids, bias_values=self.bias_values, allowed_bitmask=self.allowed)
 
     def step(self) -> None:
+        """Appends a token to each history; of a full one it replaces the last."""
         token = self.scores().argmax(1)
-        self.token_ids.scatter_(1, self.seq_lens.long().unsqueeze(1), token.int().unsqueeze(1))
-        self.seq_lens += 1
+        room = self.token_ids.shape[1]
+        self.token_ids.scatter_(1, self.seq_lens.long().clamp(max=room - 1).unsqueeze(1), token.int().unsqueeze(1))
+        self.seq_lens.add_(1).clamp_(max=room)
 
     def capture(self) -> torch.cuda.CUDAGraph:
         """A graph of one step; capturing leaves the histories as they are."""

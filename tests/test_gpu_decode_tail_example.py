@@ -101,3 +101,21 @@ def test_main_runs(capsys):
     answers = _example().main(["--requests", "2", "--steps", "6", "--vocab", "2048"])
     assert [len(a) for a in answers] == [6, 6]
     assert "us a step" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_past_a_full_history_stay_inside_it(captured):
+    t = _example().DecodeTail(requests=3, hidden=256, experts=8, top_k=2, inner=128, shared=128, vocab=600, max_len=4)
+    step = t.capture().replay if captured else t.step
+    for _ in range(3):
+        step()
+    assert t.seq_lens.tolist() == [4] * 3
+    full = t.token_ids.clone()
+    for _ in range(5):
+        step()
+    assert t.seq_lens.tolist() == [4] * 3 and torch.equal(t.token_ids[:, :3], full[:, :3])
+    assert ((t.token_ids >= 0) & (t.token_ids < 600)).all()
+
+
+def test_main_without_steps():
+    assert _example().main(["--requests", "2", "--steps", "0", "--vocab", "2048"]) == [[], []]
