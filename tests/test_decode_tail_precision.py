@@ -362,3 +362,28 @@ def test_moe_route_of_very_many_rows():
     ids, w = _ops().moe_route(x, wr, 2)
     last, lw = _ops().moe_route(x[-40:], wr, 2)
     assert torch.equal(ids[-40:], last) and torch.equal(w[-40:], lw)
+
+
+# ---------------------------------------------------------------------------
+# refusals
+# ---------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("name", ["repetition", "frequency", "presence", "bias_ids"])
+def test_a_number_for_all_requests_is_refused(name):
+    """As the other arguments are, with a ValueError and the logits untouched."""
+    x = torch.ones((3, 40), device="cuda")
+    one = torch.tensor(1, dtype=torch.int32 if name == "bias_ids" else torch.float32, device="cuda")
+    with pytest.raises(ValueError):
+        _ops().apply_logit_penalties(x, **{name: one}, **({"bias_values": one.float()} if name == "bias_ids" else {}))
+    assert (x == 1).all()
+
+
+@gpu
+def test_experts_without_a_stack_are_refused():
+    x = torch.zeros((2, 64), device="cuda", dtype=torch.bfloat16)
+    ids, weights = torch.zeros((2, 1), device="cuda", dtype=torch.int32), torch.ones((2, 1), device="cuda")
+    for w13 in (torch.tensor(1.0, device="cuda", dtype=torch.bfloat16), torch.zeros((128, 64), device="cuda", dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            _ops().moe_experts(x, ids, weights, _ops().MoEWeights(w13, torch.zeros((64, 64), device="cuda", dtype=torch.bfloat16)))

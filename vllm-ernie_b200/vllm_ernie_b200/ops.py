@@ -611,7 +611,8 @@ def w4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zero
 
     ``x`` ``[T, K]`` bf16 or fp16; ``qweight`` uint8 ``[N, K / 2]`` (low nibble
     = even k); ``scales`` ``[N, K / g]`` of x's type, g = 32, 64 or 128;
-    ``zeros`` uint8 ``[N, K / g]`` (None: 8).  ``w = (q - zero) * scale``, sums
+    ``zeros`` uint8 ``[N, K / g]`` (None: 8), codes starting on 16 bytes, scales and
+    zeros on 4.  ``w = (q - zero) * scale``, sums
     in fp32, one rounding to x's type.  A bf16 ``|x|`` of 2^48 and more counts as
     infinite, below 2^-73 terms lose bits; an infinite or NaN ``x`` makes its own
     row infinite or NaN.  ``out`` must not overlap ``x``.  Right
@@ -748,6 +749,8 @@ _NO_SHARED = (None,) * 6
 
 def _moe_args(hidden: int, dev: int, experts: MoEWeights, shared: MoEWeights | None):
     """Checked ``(format, group, weight addresses, E, I, Is)``."""
+    if experts[0].dim() != 3:
+        _refuse("w13 must be [E, 2 I, H]")
     num = experts[0].shape[0]
     fmt, group, inner, ptrs = _moe_weights(experts, (num,), hidden, dev)
     if shared is None:
@@ -903,6 +906,8 @@ def apply_logit_penalties(logits: torch.Tensor, token_ids: torch.Tensor | None =
     reqs = rows
     for t in (token_ids, repetition, frequency, presence, bias_ids):
         if t is not None:
+            if not t.dim():
+                _refuse("token_ids, penalties and bias_ids have a row or a value a request")
             reqs = t.shape[0]
             break
     at = [0, 0, 0]  # addresses of the penalties
