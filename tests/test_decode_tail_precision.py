@@ -138,6 +138,20 @@ def test_w4_linear_of_long_rows(tokens, n, k, group, zeros, dtype):
         assert torch.equal(again, got[0])
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (64, True), (128, True)])
+@pytest.mark.parametrize("tokens,n,k", [
+    (1, 3000, 640), (2, 2500, 4224), (3, 2000, 8192), (4, 1500, 16384), (5, 1003, 8192), (8, 800, 16384), (9, 700, 4096),
+    (16, 513, 8192), (17, 300, 2176), (33, 200, 8192), (3, 1201, 24576), (2, 700, 32768)])
+def test_w4_linear_rounds_once(tokens, n, k, group, zeros, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(n + k)
+    x = torch.randn((tokens, k), generator=gen, device="cuda").to(dtype)
+    q, s, z = _w4_weights(n, k, group, zeros, dtype, gen, "cuda")
+    ref, size = _w4_ref(x, q, s, z, group)
+    assert _w4_holds(_ops().w4_linear(x, q, s, z), ref, size, dtype, k // group)
+
+
 # ---------------------------------------------------------------------------
 # experts
 # ---------------------------------------------------------------------------
@@ -187,7 +201,7 @@ def _experts_ref(x, ids, weights, w13, w2, shared=None):
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "w4-32", "w4-64z", "w4-128"])
 @pytest.mark.parametrize("tokens,experts,hidden,inner,shared", [
     (1, 4, 1024, 256, 384), (2, 4, 1024, 384, 128), (3, 4, 1024, 256, 384), (4, 6, 1024, 384, 128), (5, 6, 1024, 256, 384),
-    (8, 6, 512, 384, 640), (9, 20, 512, 256, 384), (16, 3, 512, 384, 256), (40, 6, 512, 256, 384), (70, 12, 512, 128, 0)])
+    (8, 6, 512, 384, 640), (9, 20, 512, 256, 384), (16, 3, 512, 384, 256), (40, 6, 512, 256, 384), (70, 12, 512, 128, 0), (5, 6, 8192, 256, 0), (12, 4, 1024, 8192, 384)])
 def test_moe_experts_round_once(tokens, experts, hidden, inner, shared, kind):
     """The gated product between the two products is not rounded to bf16: with it
     in one number the error is that of two roundings.  All widths of columns, with
@@ -200,6 +214,20 @@ def test_moe_experts_round_once(tokens, experts, hidden, inner, shared, kind):
     weights = torch.rand((tokens, 3), generator=gen, device="cuda")
     got = _ops().moe_experts(x, ids, weights, stack, shared=one)
     assert _rounded_once(got, _experts_ref(x, ids, weights, w13, w2, (a, b) if shared else None), torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "w4-32"])
+@pytest.mark.parametrize("tokens,hidden,inner,shared", [(5, 2080, 736, 96), (2, 2080, 160, 736), (13, 1056, 96, 32), (3, 4128, 32, 4096)])
+def test_moe_experts_of_odd_sizes_round_once(tokens, hidden, inner, shared, kind):
+    gen = _gen(tokens + hidden)
+    x = torch.randn((tokens, hidden), generator=gen, device="cuda").bfloat16()
+    stack, w13, w2 = _stack(kind, (4,), hidden, inner, gen)
+    one, a, b = _stack(kind, (), hidden, shared, gen)
+    ids = torch.randint(-1, 4, (tokens, 3), generator=gen, device="cuda", dtype=torch.int32)  # skipped and repeated ones too
+    weights = torch.rand((tokens, 3), generator=gen, device="cuda")
+    got = _ops().moe_experts(x, ids, weights, stack, shared=one)
+    assert _rounded_once(got, _experts_ref(x, ids, weights, w13, w2, (a, b)), torch.bfloat16)
 
 
 @gpu
