@@ -126,6 +126,7 @@ def test_the_rounding_check_tells_one_bf16_number_from_two(inner):
     (1, 20000, 29568, 32),
     (2, 10000, 37504, 64),
     (9, 8192, 43136, 128),
+    (2, 8192, 33792, 32),     # the last piece's scales in whole 16 bytes
 ])
 def test_w4_linear_of_long_rows(tokens, n, k, group, zeros, dtype):
     gen = torch.Generator(device="cuda").manual_seed(n + k)
@@ -277,6 +278,45 @@ def test_an_e4m3_nan_is_a_nan(tokens, hidden, inner, value):
 # ---------------------------------------------------------------------------
 # the range of bf16 activations
 # ---------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("tokens,experts", [(1, 3), (4, 3), (40, 20), (64, 4), (70, 5)])
+def test_an_e4m3_nan_in_any_block_and_in_the_shared_expert(tokens, experts):
+    gen = _gen(tokens + experts)
+    hidden, inner, shared = 384, 256, 160
+    x = torch.randn((tokens, hidden), generator=gen, device="cuda").bfloat16()
+    stack, _, _ = _stack("fp8", (experts,), hidden, inner, gen)
+    one, _, _ = _stack("fp8", (), hidden, shared, gen)
+    ids = torch.randint(0, experts, (tokens, 2), generator=gen, device="cuda", dtype=torch.int32)
+    weights = torch.rand((tokens, 2), generator=gen, device="cuda")
+
+    def run(w, sh):
+        return _ops().moe_experts(x, ids, weights, w, shared=sh)
+
+    def with_nan(w, *at):
+        w = w.clone()
+        w.view(torch.uint8)[at] = 0x7F
+        return w
+
+    clean = run(stack, one)
+    e = int(ids[tokens // 2, 1])
+    has = (ids == e).any(1)
+    got = run(stack._replace(w13=with_nan(stack.w13, e, 11, 300)), one)
+    assert torch.isnan(got[has]).all() and torch.equal(got[~has], clean[~has])
+    got = run(stack._replace(w2=with_nan(stack.w2, e, 380, 31)), one)
+    assert torch.isnan(got[has, 380]).all() and torch.isnan(got).sum() == has.sum()
+    keep = ~torch.isnan(got)
+    assert torch.equal(got[keep], clean[keep])
+    assert torch.isnan(run(stack, one._replace(w13=with_nan(one.w13, 2 * shared - 1, 5)))).all()
+    got = run(stack, one._replace(w2=with_nan(one.w2, 7, 159)))
+    assert torch.isnan(got[:, 7]).all() and torch.isnan(got).sum() == tokens
+    # two experts at once, and none left over for the next call
+    bad = with_nan(with_nan(stack.w13, 0, 0, 0), experts - 1, 2 * inner - 1, hidden - 1)
+    has = (ids == 0).any(1) | (ids == experts - 1).any(1)
+    got = run(stack._replace(w13=bad), one)
+    assert torch.equal(torch.isnan(got).all(1), has) and torch.equal(got[~has], clean[~has])
+    assert torch.equal(run(stack, one), clean)
 
 
 @gpu
