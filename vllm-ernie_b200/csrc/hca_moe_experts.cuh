@@ -3,8 +3,8 @@
 //   h[t, j] = w[t, j] silu(W1_e x_t) * (W3_e x_t),  e = ids[t, j]
 //   y[t]    = sum_j W2_e h[t, j]  (+ the shared expert's with weight 1)
 //
-// Both products are bound by the bytes of the chosen experts' weights, each
-// read once for all tokens that chose the expert (hca_stream.cuh).  A CTA of
+// Both products go through the chosen experts' weights, each read once for a
+// block of columns of the tokens that chose the expert (hca_stream.cuh).  A CTA of
 // 16 warps takes a contiguous run of (expert, 16 rows) tiles, so that it meets
 // few experts and lays out their columns in shared memory once.  The second
 // product leaves each (token, slot) pair's share of y in 32 bits, and the last
@@ -19,10 +19,12 @@
 // token: the weights of the second product start on their way before the
 // barrier that its activations wait for.
 //
-// Measured, router and all: e4m3, 8 tokens, 8 of 128 experts, 4096 x 1024 and a
-// shared one: 118 us, 5.6 TB/s; bf16, one token, 6 of 64: 37.9 us, 4.0 TB/s;
-// 4-bit, 64 tokens, 8 of 128: 193 us, 4.2 TB/s, bound by latency at 16 warps an
-// SM (weights and the groups' barriers are two fifths of what warps wait for).
+// Measured, router and all, and the rate by the bytes of the chosen experts: e4m3,
+// 8 tokens, 8 of 128 experts (41 different ones), 4096 x 1024 and a shared one: 122
+// us, 4.4 TB/s; bf16, one token, 6 of 64: 37.6 us, 4.0 TB/s; 4-bit, 59 tokens, 8 of
+// 128 (83): 192 us, 2.8 TB/s, since experts with more than eight tokens are read
+// for each eight (649 MB instead of 547).  Bound by latency at 16 warps an SM:
+// waiting for loads and at the groups' barriers, no pipe above two thirds.
 // Of a small layer's 18 us (4-bit, 2 tokens, 4 of 32, 1024 x 512), 3 are the
 // router, 3 the plan, 3 1/2 the starts of the products, 6 the products and 2 1/2
 // the barriers.

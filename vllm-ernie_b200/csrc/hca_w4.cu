@@ -8,13 +8,14 @@
 // sums meet in shared memory in warp order, so results do not depend on
 // timing.
 //
-// Measured: [129281, 4096], groups of 128 with zero points, 8 rows: 53.4 us,
+// Measured: [129281, 4096], groups of 128 with zero points, 8 rows: 53.6 us,
 // 5.2 TB/s (a run of seconds meets the power limit: 61 us at 1.65 GHz; the loop
 // keeps the issue slots half and the shared-memory pipe two thirds busy).  Small
 // ones are bound by what comes before the first product, laying out x above all
-// (16 rows of 4096: about 2 us of 10.0 for [8192, 4096]), and with groups of 32 by
-// the unpacking (fp16, [4096, 8192], 3 rows: 10.1 us); [8192, 1024], one row:
-// 3.8 us.
+// (16 rows of 4096: about 2 us of 10.2 for [8192, 4096]), and by uneven shares
+// (fp16, [4096, 8192], 3 rows, groups of 32: 10.1 us, 256 tiles on 148 SMs, issue
+// slots half full); [8192, 1024], one row: 3.8 us.  Rows in pieces: 3 x 29568,
+// N 8192, groups of 32: 101 us for 22 of bytes.
 #include "hca_stream.cuh"
 
 #include <algorithm>
